@@ -15,7 +15,7 @@ CBK_ERR_INVALID = -1
 CBK_ERR_UNSUPPORTED = -2
 CBK_ERR_CUDA = -3
 CBK_ERR_WORKSPACE = -4
-CBK_BF16, CBK_F16 = 0, 1
+CBK_BF16, CBK_F16, CBK_F32 = 0, 1, 2
 CBK_ROPE_REF, CBK_ROPE_FP32 = 0, 1
 CBK_ROPE_TABLE_BY_ROW = 16
 CBK_STATUS_BAD_INDEX, CBK_STATUS_TIMEOUT, CBK_STATUS_COUNT = 1, 2, 4
@@ -53,6 +53,14 @@ SIGNATURES = {
     "cbk_decode_attn_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
     "cbk_decode_attn": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _f32, _i32, _vp, _vp, _sz,
                                _vp, _vp]),
+    "cbk_norm_rope_scatter": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32,
+                                     _i32, _vp, _vp, _f32, _vp, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "cbk_tree_attn_workspace_bytes": (_sz, [_i32, _i64, _i32, _i32, _i32]),
+    "cbk_tree_attn": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _f32, _i32, _vp,
+                             _vp, _sz, _vp, _vp]),
+    "cbk_process_logits": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _f32, _f32,
+                                  _f32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _i64, _vp, _vp,
+                                  _vp]),
 }
 
 

@@ -486,3 +486,294 @@ def scatter_rows(src: torch.Tensor, idx: torch.Tensor, n_rows: int, out: torch.T
                                        o2.stride(0) * o2.element_size(), int(n_rows), row_bytes, _stream(dev)),
                 "cbk_scatter_rows")
     return out
+
+
+# ---------------------------------------------------------------------------
+# decoding with drafted tokens
+# ---------------------------------------------------------------------------
+_DT3 = {**_DT, torch.float32: N.CBK_F32}
+
+
+def _call(name: str, dev: torch.device, n_launches: int, *args) -> None:
+    """One C-ABI call on dev's current stream (the stream is appended), with dev
+    the current device meanwhile and its span timed when timing is on."""
+    fn = getattr(N.LIB, "cbk_" + name)
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    if TIMES.active or torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev), TIMES.span(name, dev, n_launches):
+            rc = fn(*args, stream)
+    else:
+        rc = fn(*args, stream)
+    if rc:
+        N.check(rc, "cbk_" + name)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _src_rows(t: torch.Tensor, n: int, cols: int, who: str) -> torch.Tensor:
+    """t as n rows of cols elements, in place where its rows can be read as they are."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.shape[0] != n or t.shape[1] != cols:
+        raise ValueError(f"{who} must be {n} rows of {cols}, got {list(t.shape)}")
+    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < cols or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _index(t: torch.Tensor, n: int, who: str) -> torch.Tensor:
+    if t.dtype != torch.int64 or t.numel() != n:
+        raise ValueError(f"{who} must be int64 with {n} entries, got {t.dtype}{list(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, kv_dim: int, who: str) -> None:
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise ValueError(f"{who}: caches must be {dtype}, got {k_cache.dtype} / {v_cache.dtype}")
+    if (k_cache.dim() != 2 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride()
+            or k_cache.shape[1] != kv_dim or k_cache.stride(1) != 1):
+        raise ValueError(f"{who}: k_cache and v_cache must be rows of {kv_dim} elements with one layout, got "
+                         f"{list(k_cache.shape)} and {list(v_cache.shape)}")
+
+
+def norm_rope_scatter(q_src: torch.Tensor, k_src: torch.Tensor, v_src: torch.Tensor, positions: torch.Tensor,
+                      rows: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim: int, rope: torch.Tensor,
+                      k_cache: torch.Tensor, v_cache: torch.Tensor, q_weight: torch.Tensor | None = None,
+                      k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
+                      q_out: torch.Tensor | None = None, mode: str = "ref", status=None) -> torch.Tensor:
+    """Per-head RMSNorm (with ``q_weight`` and ``k_weight``) and rotation of Q and K
+    at ``positions``; K and V into cache rows ``rows``.  Returns the rotated Q,
+    [n][Hq*D].
+
+    q_src / k_src / v_src: n rows of heads (views of one stacked projection are
+    read in place); ``positions`` and ``rows``: int64, n entries -- siblings of a
+    drafted tree share a position, not a row; rows are distinct, and a row of -1
+    marks a padding token of which nothing is written.  ``rope``: fp32 (cos, sin)
+    table [n_pos][R / 2][2]; the first R dimensions of a head are rotated, as the
+    pairs (i, i + R / 2) or, ``interleaved``, (2i, 2i + 1).  k_cache / v_cache:
+    [cap][Hkv*D].  ``mode`` "ref" rounds to 16 bits where the HF modules do, "fp32"
+    once.  A position or row outside its buffer sets CBK_STATUS_BAD_INDEX and
+    skips the token."""
+    dev = require_cuda(q_src, k_src, v_src, positions, rows, rope, k_cache, v_cache, q_weight, k_weight, q_out,
+                       status)
+    dt = q_src.dtype
+    code = dtype_code(dt)
+    if mode not in ROPE_MODES:
+        raise ValueError(f"norm_rope_scatter: mode must be one of {sorted(ROPE_MODES)}, got {mode!r}")
+    if k_src.dtype != dt or v_src.dtype != dt:
+        raise ValueError(f"norm_rope_scatter: q, k and v must have one dtype, got {dt}, {k_src.dtype}, {v_src.dtype}")
+    n, qd, kd = rows.numel(), n_q_heads * head_dim, n_kv_heads * head_dim
+    q2 = _src_rows(q_src, n, qd, "norm_rope_scatter: q_src")
+    k2 = _src_rows(k_src, n, kd, "norm_rope_scatter: k_src")
+    v2 = _src_rows(v_src, n, kd, "norm_rope_scatter: v_src")
+    positions = _index(positions, n, "norm_rope_scatter: positions")
+    rows = _index(rows, n, "norm_rope_scatter: rows")
+    if rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or not rope.is_contiguous():
+        raise ValueError("norm_rope_scatter: rope must be a contiguous fp32 table [n_pos][R / 2][2]")
+    _check_cache(k_cache, v_cache, dt, kd, "norm_rope_scatter")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("norm_rope_scatter: give both q_weight and k_weight, or neither")
+    if q_weight is not None:
+        for w in (q_weight, k_weight):
+            if w.dtype != dt or w.numel() != head_dim or not w.is_contiguous():
+                raise ValueError(f"norm_rope_scatter: weights must be contiguous {dt}[{head_dim}], got "
+                                 f"{w.dtype}{list(w.shape)}")
+    if q_out is None:
+        q_out = torch.empty((n, qd), dtype=dt, device=dev)
+    elif q_out.dtype != dt or q_out.numel() != n * qd or not q_out.is_contiguous():
+        raise ValueError(f"norm_rope_scatter: q_out must be contiguous {dt} with {n} rows of {qd}")
+    _call("norm_rope_scatter", dev, 1, q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), v2.data_ptr(),
+          v2.stride(0), positions.data_ptr(), rows.data_ptr(), n, n_q_heads, n_kv_heads, head_dim,
+          2 * rope.shape[1], int(bool(interleaved)), code, _ptr(q_weight), _ptr(k_weight), eps, rope.data_ptr(),
+          rope.shape[0], ROPE_MODES[mode], q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+          k_cache.stride(0), k_cache.shape[0], _ptr(status))
+    return q_out
+
+
+def tree_workspace(n_nodes: int, cap: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """Workspace of tree_attn for up to n_nodes nodes over a cache of cap rows
+    (reusable by calls that do not overlap on the GPU)."""
+    if head_dim not in (64, 128) or n_nodes > 1024:
+        raise NotImplementedError(f"tree_attn: head_dim 64 or 128 and at most 1024 nodes, got {head_dim}, {n_nodes}")
+    device = torch.device(device)
+    with torch.cuda.device(device):
+        nbytes = N.LIB.cbk_tree_attn_workspace_bytes(n_nodes, cap, n_q_heads, n_kv_heads, head_dim)
+    if nbytes == 0:
+        raise ValueError(f"tree_workspace: {N.last_error()}")
+    return torch.empty((nbytes,), dtype=torch.uint8, device=device)
+
+
+def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_ctx: torch.Tensor,
+              words: torch.Tensor, n_q_heads: int, n_kv_heads: int, head_dim: int, scale: float,
+              workspace: torch.Tensor | None = None, out: torch.Tensor | None = None, status=None) -> torch.Tensor:
+    """Attention of a tree of T drafted tokens over cache rows [0, n_ctx) and the
+    nodes' own rows n_ctx + j, of which node i sees those with bit j of
+    ``words[i]`` set (int32 [T][>= ceil(T / 32)], bit j % 32 of word j / 32; see
+    ``tree_words``).  q: [T][Hq*D] (rotated); ``n_ctx``: one int64 on the device,
+    so that a captured step stays valid as it advances; returns [T][Hq*D].  A
+    node that sees no row gets zeros; masked rows and rows behind the tree may
+    hold anything.  n_ctx + T beyond the cache sets CBK_STATUS_BAD_INDEX and
+    leaves ``out`` as it was."""
+    dev = require_cuda(q, k_cache, v_cache, n_ctx, words, workspace, out, status)
+    dt = q.dtype
+    code = dtype_code(dt)
+    t, qd = words.shape[0], n_q_heads * head_dim
+    if words.dtype != torch.int32 or words.dim() != 2 or words.shape[1] * 32 < t or words.stride(1) != 1:
+        raise ValueError(f"tree_attn: words must be int32 [T][>= ceil(T / 32)] rows, got "
+                         f"{words.dtype}{list(words.shape)}")
+    if q.numel() != t * qd or q.shape[-1] != qd:
+        raise ValueError(f"tree_attn: q must be {t} rows of {qd}, got {list(q.shape)}")
+    if n_ctx.dtype != torch.int64 or n_ctx.numel() != 1:
+        raise ValueError("tree_attn: n_ctx must be one int64 on the device")
+    _check_cache(k_cache, v_cache, dt, n_kv_heads * head_dim, "tree_attn")
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    words, words_stride = _word_rows(words)
+    cap = k_cache.shape[0]
+    if workspace is None:
+        workspace = tree_workspace(t, cap, n_q_heads, n_kv_heads, head_dim, dev)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("tree_attn: workspace must come from tree_workspace")
+    if out is None:
+        out = torch.empty((t, qd), dtype=dt, device=dev)
+    elif out.dtype != dt or out.numel() != t * qd or not out.is_contiguous():
+        raise ValueError(f"tree_attn: out must be contiguous {dt} with {t} rows of {qd}")
+    _call("tree_attn", dev, 1, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0),
+          n_ctx.data_ptr(), words.data_ptr(), words_stride, t, cap, n_q_heads, n_kv_heads, head_dim, scale, code,
+          out.data_ptr(), workspace.data_ptr(), workspace.numel(), _ptr(status))
+    return out
+
+
+def tree_words(parents: Sequence[int], width: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(words, depth) of a drafted tree given each node's parent (-1 for a root,
+    else an earlier node): words int32 [T][width] (default ceil(T / 32)) with bit
+    j of row i set for node i and its ancestors, depth int64 [T] (0 for a root);
+    both on the host."""
+    n = len(parents)
+    need = max(1, (n + 31) // 32)
+    width = need if width is None else width
+    if width < need:
+        raise ValueError(f"tree_words: {n} nodes need {need} words, got width {width}")
+    seen = np.zeros((n, 32 * width), dtype=np.uint8)
+    depth = np.zeros((n,), dtype=np.int64)
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError(f"tree_words: node {i} has parent {p} (-1 or an earlier node)")
+        if p >= 0:
+            seen[i] = seen[p]
+            depth[i] = depth[p] + 1
+        seen[i, i] = 1
+    words = np.packbits(seen, axis=1, bitorder="little").view("<i4").astype(np.int32)
+    return torch.from_numpy(words), torch.from_numpy(depth)
+
+
+def _word_rows(words: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """2-D bit words and their row stride; broadcast or overlapping rows are copied apart."""
+    if words.shape[0] <= 1:
+        return words, words.shape[1]
+    if words.stride(0) < words.shape[1]:
+        words = words.contiguous()
+    return words, words.stride(0)
+
+
+def _row_stride(t: torch.Tensor, rows: int, cols: int, who: str) -> tuple[torch.Tensor, int]:
+    """t as [rows][>= cols] or one shared row; (tensor with unit inner stride, row stride or 0)."""
+    if t.dim() == 1:
+        t = t.unsqueeze(0)
+    if t.dim() != 2 or t.shape[0] not in (1, rows) or t.shape[1] < cols:
+        raise ValueError(f"{who} must be one row or {rows} rows of at least {cols}, got {list(t.shape)}")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        t = t.contiguous()
+    return t, (0 if t.shape[0] == 1 else t.stride(0))
+
+
+def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                   n_prompt: torch.Tensor | None = None, repetition: float = 1.0, presence: float = 0.0,
+                   frequency: float = 0.0, bias: torch.Tensor | None = None, mask_words: torch.Tensor | None = None,
+                   tree_tokens: torch.Tensor | None = None, tree_words: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None, return_logits: bool = True,
+                   status=None):
+    """Penalties for repeated tokens, bias and grammar mask on rows of logits, and
+    the token each row chooses: (processed logits or None, int64 tokens).
+
+    logits: [rows][vocab] bf16, fp16 or fp32 (leading dimensions are kept).
+    ``history``: int64 token ids, one row for all or one per row, of which the
+    first ``lengths`` (int64 on the device, one or one per row; default all) count
+    and the first ``n_prompt`` of those are the prompt's (default none); the rest
+    were made.  With ``tree_tokens`` / ``tree_words`` row r is a node of a drafted
+    tree and the tokens on its path were made too.  A token made c times or in
+    the prompt: x / repetition if x > 0, else x * repetition; made: x - frequency *
+    c - presence; then ``bias`` (fp32, one row or one per row) and, where
+    ``mask_words`` (int32, bit t % 32 of word t / 32) has a clear bit, -inf.  The
+    token is the first largest value (NaN counts as largest); a row of -inf
+    chooses 0.  ``out`` may be ``logits``; ``out_dtype`` is the logits' (default)
+    or fp32."""
+    dev = require_cuda(logits, history, lengths, n_prompt, bias, mask_words, tree_tokens, tree_words, out, status)
+    if logits.dtype not in _DT3:
+        raise NotImplementedError(f"process_logits: bf16, fp16 or fp32 logits, got {logits.dtype}")
+    shape = logits.shape
+    if logits.dim() != 2:
+        logits = logits.reshape(-1, shape[-1])
+    rows, vocab = logits.shape
+    if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
+        logits = logits.contiguous()
+    hist_stride = hist_cap = len_stride = prompt_stride = bias_stride = mask_stride = tree_stride = n_tree = 0
+    if history is None and (lengths is not None or n_prompt is not None):
+        raise ValueError("process_logits: lengths and n_prompt belong to a history")
+    if (tree_tokens is None) != (tree_words is None):
+        raise ValueError("process_logits: give both tree_tokens and tree_words, or neither")
+    if history is not None:
+        if history.dtype != torch.int64:
+            raise ValueError(f"process_logits: history must be int64, got {history.dtype}")
+        history, hist_stride = _row_stride(history, rows, 0, "process_logits: history")
+        hist_cap = history.shape[1]
+        if lengths is not None:
+            lengths = _index(lengths, 1 if lengths.numel() == 1 else rows, "process_logits: lengths")
+            len_stride = int(lengths.numel() != 1)
+        if n_prompt is not None:
+            n_prompt = _index(n_prompt, 1 if n_prompt.numel() == 1 else rows, "process_logits: n_prompt")
+            prompt_stride = int(n_prompt.numel() != 1)
+    if tree_tokens is not None:
+        n_tree = tree_tokens.numel()
+        tree_tokens = _index(tree_tokens, n_tree, "process_logits: tree_tokens")
+        if (tree_words.dtype != torch.int32 or tree_words.dim() != 2 or tree_words.shape[0] != rows
+                or tree_words.shape[1] * 32 < n_tree or tree_words.stride(1) != 1):
+            raise ValueError(f"process_logits: tree_words must be int32, {rows} rows of at least {n_tree} bits")
+        tree_words, tree_stride = _word_rows(tree_words)
+    if bias is not None:
+        if bias.dtype != torch.float32:
+            raise ValueError(f"process_logits: bias must be fp32, got {bias.dtype}")
+        bias, bias_stride = _row_stride(bias, rows, vocab, "process_logits: bias")
+    if mask_words is not None:
+        if mask_words.dtype != torch.int32:
+            raise ValueError(f"process_logits: mask_words must be int32, got {mask_words.dtype}")
+        mask_words, mask_stride = _row_stride(mask_words, rows, (vocab + 31) // 32, "process_logits: mask_words")
+    out2 = None
+    if out is not None:
+        if out_dtype not in (None, out.dtype):
+            raise ValueError(f"process_logits: out is {out.dtype}, out_dtype {out_dtype}")
+        if out.numel() != rows * vocab or out.shape[-1] != vocab:
+            raise ValueError(f"process_logits: out must be {rows} rows of {vocab}, got {list(out.shape)}")
+        out2 = out.view(-1, vocab)
+        if out2.stride(1) != 1:
+            raise ValueError("process_logits: out rows must be contiguous")
+    elif return_logits:
+        out = torch.empty(shape, dtype=out_dtype or logits.dtype, device=dev)
+        out2 = out if len(shape) == 2 else out.view(-1, vocab)
+    tokens = torch.empty(shape[:-1], dtype=torch.int64, device=dev)
+    if out2 is not None and out2.dtype not in _DT3:
+        raise NotImplementedError(f"process_logits: bf16, fp16 or fp32 output, got {out2.dtype}")
+    if not (repetition > 0 and presence == presence and frequency == frequency):
+        raise ValueError("process_logits: repetition must be > 0 and no penalty NaN")
+    if repetition == 1.0 and presence == 0.0 and frequency == 0.0:
+        hist_cap = n_tree = 0                    # nothing depends on the counts
+    _call("process_logits", dev, 1, logits.data_ptr(), _DT3[logits.dtype], logits.stride(0) if rows > 1 else vocab,
+          rows, vocab, _ptr(history), hist_stride, hist_cap, _ptr(lengths), len_stride, _ptr(n_prompt), prompt_stride,
+          repetition, presence, frequency, _ptr(bias), bias_stride, _ptr(mask_words), mask_stride, _ptr(tree_tokens),
+          _ptr(tree_words), tree_stride, n_tree, _ptr(out2), _DT3[out2.dtype] if out2 is not None else 0,
+          (out2.stride(0) if rows > 1 else vocab) if out2 is not None else 0, tokens.data_ptr(), _ptr(status))
+    return out, tokens

@@ -46,7 +46,8 @@ enum {
   CBK_ERR_WORKSPACE = -4     /* caller workspace too small */
 };
 
-enum { CBK_BF16 = 0, CBK_F16 = 1 };
+/* CBK_F32 only where an entry says so (cbk_process_logits). */
+enum { CBK_BF16 = 0, CBK_F16 = 1, CBK_F32 = 2 };
 
 /* RoPE rounding modes for K/Q rotation.
  * CBK_ROPE_REF:  reproduce HF `apply_rotary_pos_emb` on 16-bit tensors: cos/sin
@@ -253,6 +254,81 @@ int cbk_decode_attn(const void* q, const void* k_cache, const void* v_cache, int
  * [0, S); rows of row_bytes (multiple of 16), 16-byte aligned, byte strides. */
 int cbk_scatter_rows(const void* src, int64_t src_stride_bytes, const int64_t* idx, int64_t k, void* dst,
                      int64_t dst_stride_bytes, int64_t S, int64_t row_bytes, void* stream);
+
+/* Decoding with drafted tokens: the three entries below, in this order, are one
+ * layer's and one step's work beside its GEMMs when a model checks a tree of
+ * drafted tokens at once instead of one token (no counterpart in the reference,
+ * whose decode loop, runners.py:106-152, takes one token at a time).
+ *
+ * cbk_norm_rope_scatter: per-head RMSNorm of Q and K (when q_weight and k_weight,
+ * head_dim elements each, are given), rotation, and K / V into their cache rows.
+ * For token j < n with p = positions[j], r = rows[j]:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight            per head of q_src[j], k_src[j]
+ *   (y_a, y_b) -> (y_a c - y_b s, y_b c + y_a s)       (c, s) = rope_table[p][i],
+ *     i < rotary_dim / 2, (a, b) = (i, i + rotary_dim / 2) or, interleaved,
+ *     (2i, 2i + 1); dimensions from rotary_dim on are not rotated
+ *   q_out[j] = q, k_cache[r] = k, v_cache[r] = v_src[j]
+ * rope_table: float2[table_rows][rotary_dim / 2].  Source and cache row strides
+ * in elements; q_out is [n][n_q_heads * head_dim] and must not overlap a source.
+ * rope_mode: CBK_ROPE_REF rounds to 16 bits where the HF modules do,
+ * CBK_ROPE_FP32 once.  A row of -1 marks a padding token (nothing of it is
+ * written); any other position or row outside its buffer sets
+ * CBK_STATUS_BAD_INDEX and skips the token.  Rows are distinct (of two tokens with
+ * one row, either's values may land).  head_dim and rotary_dim multiples of 16,
+ * 16 <= rotary_dim <= head_dim <= 256; pointers 16-byte aligned, strides
+ * multiples of 8. */
+int cbk_norm_rope_scatter(const void* q_src, int64_t q_row_stride, const void* k_src, int64_t k_row_stride,
+                          const void* v_src, int64_t v_row_stride, const int64_t* positions, const int64_t* rows,
+                          int64_t n, int n_q_heads, int n_kv_heads, int head_dim, int rotary_dim, int interleaved,
+                          int dtype, const void* q_weight, const void* k_weight, float eps, const void* rope_table,
+                          int64_t table_rows, int rope_mode, void* q_out, void* k_cache, void* v_cache,
+                          int64_t kv_row_stride, int64_t cap, int32_t* status, void* stream);
+
+/* Attention of a tree of drafted tokens over the cache.  Node i < n_nodes sees
+ * rows [0, *n_ctx) and row *n_ctx + j for every j with bit j % 32 of
+ * words[i][j / 32] set (its ancestors and itself; the nodes' own K and V are in
+ * those rows):
+ *   out[i][h] = softmax_t(scale * q[i][h] . k[t][h / G]) . v[t][h / G]
+ * q, out: [n_nodes][n_q_heads][head_dim]; caches: cap rows of kv_row_stride
+ * elements, head h at h * head_dim; words: rows of words_stride int32.  A node
+ * that sees no row gets zeros.  What a masked row holds (NaN and infinities
+ * included) and rows from *n_ctx + n_nodes on do not matter.  *n_ctx is read on
+ * the device (a captured graph stays valid as it advances); *n_ctx < 0 or
+ * *n_ctx + n_nodes > cap sets CBK_STATUS_BAD_INDEX and leaves out untouched.
+ * head_dim 64 or 128, n_nodes <= 1024, any whole number of q heads per KV head;
+ * pointers 16-byte aligned, kv_row_stride a multiple of 8.
+ * The workspace needs no initialisation; calls that overlap on the GPU must not
+ * share it. */
+size_t cbk_tree_attn_workspace_bytes(int n_nodes, int64_t cap, int n_q_heads, int n_kv_heads, int head_dim);
+int cbk_tree_attn(const void* q, const void* k_cache, const void* v_cache, int64_t kv_row_stride,
+                  const int64_t* n_ctx, const int32_t* words, int64_t words_stride, int n_nodes, int64_t cap,
+                  int n_q_heads, int n_kv_heads, int head_dim, float scale, int dtype, void* out, void* workspace,
+                  size_t workspace_bytes, int32_t* status, void* stream);
+
+/* Penalties for repeated tokens, bias and grammar mask on rows of logits, and the
+ * token each row chooses.  Row r's history is history[r][0 .. lengths[r]), of
+ * which the first n_prompt[r] are its prompt and the rest were made; with
+ * n_tree > 0 the tokens tree_tokens[j] of the bits j set in tree_words[r] were
+ * made too (row r is node r of a drafted tree).  In fp32, one rounding per step,
+ * for token t made c times:
+ *   x = logit;  t in the prompt or c > 0:  x = x > 0 ? x / repetition : x * repetition
+ *   c > 0:  x = (x - frequency * c) - presence
+ *   x = x + bias[r][t];  bit t % 32 of mask[r][t / 32] clear:  x = -inf
+ * out[r][t] = x (out may be NULL, or logits itself when the types agree) and
+ * tokens[r] = the lowest index of the largest x (NaN counts as largest; a row of
+ * -inf chooses 0).  Row strides in elements; a stride of 0 shares one row
+ * (history, lengths, n_prompt, bias, mask); NULL: no history, whole history_cap,
+ * no prompt, no bias, no mask.  in_dtype CBK_BF16 / CBK_F16 / CBK_F32; out_dtype
+ * the same or CBK_F32.  A token outside [0, vocab) is skipped and a length
+ * outside [0, history_cap] clamped, both with CBK_STATUS_BAD_INDEX.
+ * vocab <= 458752, history_cap < 2^30, n_tree <= 1024, repetition > 0. */
+int cbk_process_logits(const void* logits, int in_dtype, int64_t row_stride, int64_t rows, int64_t vocab,
+                       const int64_t* history, int64_t history_stride, int64_t history_cap, const int64_t* lengths,
+                       int64_t lengths_stride, const int64_t* n_prompt, int64_t n_prompt_stride, float repetition,
+                       float presence, float frequency, const float* bias, int64_t bias_stride, const int32_t* mask,
+                       int64_t mask_stride, const int64_t* tree_tokens, const int32_t* tree_words,
+                       int64_t tree_stride, int n_tree, void* out, int out_dtype, int64_t out_stride,
+                       int64_t* tokens, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }
