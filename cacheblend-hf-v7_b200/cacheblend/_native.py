@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libcbk.so")
 
@@ -53,14 +54,19 @@ SIGNATURES = {
     "cbk_decode_attn_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
     "cbk_decode_attn": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _f32, _i32, _vp, _vp, _sz,
                                _vp, _vp]),
-    "cbk_norm_rope_scatter": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32,
-                                     _i32, _vp, _vp, _f32, _vp, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _vp]),
+    # arguments in a packed struct (PACK)
+    "cbk_norm_rope_scatter": (_i32, [ctypes.c_char_p, _vp]),
     "cbk_tree_attn_workspace_bytes": (_sz, [_i32, _i64, _i32, _i32, _i32]),
-    "cbk_tree_attn": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _i64, _i32, _i32, _i32, _f32, _i32, _vp,
-                             _vp, _sz, _vp, _vp]),
-    "cbk_process_logits": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _f32, _f32,
-                                  _f32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _i64, _vp, _vp,
-                                  _vp]),
+    "cbk_tree_attn": (_i32, [ctypes.c_char_p, _vp]),
+    "cbk_process_logits": (_i32, [ctypes.c_char_p, _vp]),
+}
+
+
+# argument structs of include/cbk.h, fields in order (the first is the struct's size)
+PACK = {
+    "cbk_norm_rope_scatter": struct.Struct("=20q7if"),
+    "cbk_tree_attn": struct.Struct("=13q5if"),
+    "cbk_process_logits": struct.Struct("=23q3i3f"),
 }
 
 

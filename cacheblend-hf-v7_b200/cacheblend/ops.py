@@ -495,21 +495,35 @@ _DT3 = {**_DT, torch.float32: N.CBK_F32}
 
 
 def _call(name: str, dev: torch.device, n_launches: int, *args) -> None:
-    """One C-ABI call on dev's current stream (the stream is appended), with dev
-    the current device meanwhile and its span timed when timing is on."""
-    fn = getattr(N.LIB, "cbk_" + name)
+    """One C-ABI call with its packed argument struct on dev's current stream, with
+    dev the current device meanwhile and its span timed when timing is on."""
+    name_c = "cbk_" + name
+    fmt = N.PACK[name_c]
+    packed = fmt.pack(fmt.size, *args)
+    fn = getattr(N.LIB, name_c)
     stream = torch._C._cuda_getCurrentRawStream(dev.index)
     if TIMES.active or torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev), TIMES.span(name, dev, n_launches):
-            rc = fn(*args, stream)
+            rc = fn(packed, stream)
     else:
-        rc = fn(*args, stream)
+        rc = fn(packed, stream)
     if rc:
-        N.check(rc, "cbk_" + name)
+        N.check(rc, name_c)
+
+
+def _same_device(first: torch.Tensor, *others) -> torch.device:
+    """require_cuda for calls where its cost shows: the device all tensors are on."""
+    at = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != at:
+            at = -1
+    if at < 0:
+        require_cuda(first, *others)
+    return first.device
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _src_rows(t: torch.Tensor, n: int, cols: int, who: str) -> torch.Tensor:
@@ -558,7 +572,7 @@ def norm_rope_scatter(q_src: torch.Tensor, k_src: torch.Tensor, v_src: torch.Ten
     [cap][Hkv*D].  ``mode`` "ref" rounds to 16 bits where the HF modules do, "fp32"
     once.  A position or row outside its buffer sets CBK_STATUS_BAD_INDEX and
     skips the token."""
-    dev = require_cuda(q_src, k_src, v_src, positions, rows, rope, k_cache, v_cache, q_weight, k_weight, q_out,
+    dev = _same_device(q_src, k_src, v_src, positions, rows, rope, k_cache, v_cache, q_weight, k_weight, q_out,
                        status)
     dt = q_src.dtype
     code = dtype_code(dt)
@@ -586,11 +600,11 @@ def norm_rope_scatter(q_src: torch.Tensor, k_src: torch.Tensor, v_src: torch.Ten
         q_out = torch.empty((n, qd), dtype=dt, device=dev)
     elif q_out.dtype != dt or q_out.numel() != n * qd or not q_out.is_contiguous():
         raise ValueError(f"norm_rope_scatter: q_out must be contiguous {dt} with {n} rows of {qd}")
-    _call("norm_rope_scatter", dev, 1, q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), v2.data_ptr(),
-          v2.stride(0), positions.data_ptr(), rows.data_ptr(), n, n_q_heads, n_kv_heads, head_dim,
-          2 * rope.shape[1], int(bool(interleaved)), code, _ptr(q_weight), _ptr(k_weight), eps, rope.data_ptr(),
-          rope.shape[0], ROPE_MODES[mode], q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-          k_cache.stride(0), k_cache.shape[0], _ptr(status))
+    _call("norm_rope_scatter", dev, 1, q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), positions.data_ptr(),
+          rows.data_ptr(), _ptr(q_weight), _ptr(k_weight), rope.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
+          v_cache.data_ptr(), _ptr(status), q2.stride(0), k2.stride(0), v2.stride(0), k_cache.stride(0), n,
+          rope.shape[0], k_cache.shape[0], n_q_heads, n_kv_heads, head_dim, 2 * rope.shape[1], bool(interleaved), code,
+          ROPE_MODES[mode], eps)
     return q_out
 
 
@@ -618,7 +632,7 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_c
     node that sees no row gets zeros; masked rows and rows behind the tree may
     hold anything.  n_ctx + T beyond the cache sets CBK_STATUS_BAD_INDEX and
     leaves ``out`` as it was."""
-    dev = require_cuda(q, k_cache, v_cache, n_ctx, words, workspace, out, status)
+    dev = _same_device(q, k_cache, v_cache, n_ctx, words, workspace, out, status)
     dt = q.dtype
     code = dtype_code(dt)
     t, qd = words.shape[0], n_q_heads * head_dim
@@ -642,9 +656,9 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_c
         out = torch.empty((t, qd), dtype=dt, device=dev)
     elif out.dtype != dt or out.numel() != t * qd or not out.is_contiguous():
         raise ValueError(f"tree_attn: out must be contiguous {dt} with {t} rows of {qd}")
-    _call("tree_attn", dev, 1, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0),
-          n_ctx.data_ptr(), words.data_ptr(), words_stride, t, cap, n_q_heads, n_kv_heads, head_dim, scale, code,
-          out.data_ptr(), workspace.data_ptr(), workspace.numel(), _ptr(status))
+    _call("tree_attn", dev, 2, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), n_ctx.data_ptr(),
+          words.data_ptr(), out.data_ptr(), workspace.data_ptr(), _ptr(status), k_cache.stride(0), words_stride, cap,
+          workspace.numel(), t, n_q_heads, n_kv_heads, head_dim, code, scale)
     return out
 
 
@@ -712,7 +726,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, le
     token is the first largest value (NaN counts as largest); a row of -inf
     chooses 0.  ``out`` may be ``logits``; ``out_dtype`` is the logits' (default)
     or fp32."""
-    dev = require_cuda(logits, history, lengths, n_prompt, bias, mask_words, tree_tokens, tree_words, out, status)
+    dev = _same_device(logits, history, lengths, n_prompt, bias, mask_words, tree_tokens, tree_words, out, status)
     if logits.dtype not in _DT3:
         raise NotImplementedError(f"process_logits: bf16, fp16 or fp32 logits, got {logits.dtype}")
     shape = logits.shape
@@ -771,9 +785,9 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, le
         raise ValueError("process_logits: repetition must be > 0 and no penalty NaN")
     if repetition == 1.0 and presence == 0.0 and frequency == 0.0:
         hist_cap = n_tree = 0                    # nothing depends on the counts
-    _call("process_logits", dev, 1, logits.data_ptr(), _DT3[logits.dtype], logits.stride(0) if rows > 1 else vocab,
-          rows, vocab, _ptr(history), hist_stride, hist_cap, _ptr(lengths), len_stride, _ptr(n_prompt), prompt_stride,
-          repetition, presence, frequency, _ptr(bias), bias_stride, _ptr(mask_words), mask_stride, _ptr(tree_tokens),
-          _ptr(tree_words), tree_stride, n_tree, _ptr(out2), _DT3[out2.dtype] if out2 is not None else 0,
-          (out2.stride(0) if rows > 1 else vocab) if out2 is not None else 0, tokens.data_ptr(), _ptr(status))
+    _call("process_logits", dev, 1, logits.data_ptr(), _ptr(history), _ptr(lengths), _ptr(n_prompt), _ptr(bias),
+          _ptr(mask_words), _ptr(tree_tokens), _ptr(tree_words), _ptr(out2), tokens.data_ptr(), _ptr(status),
+          logits.stride(0) if rows > 1 else vocab, rows, vocab, hist_stride, hist_cap, len_stride, prompt_stride,
+          bias_stride, mask_stride, tree_stride, (out2.stride(0) if rows > 1 else vocab) if out2 is not None else 0,
+          n_tree, _DT3[logits.dtype], _DT3[out2.dtype] if out2 is not None else 0, repetition, presence, frequency)
     return out, tokens

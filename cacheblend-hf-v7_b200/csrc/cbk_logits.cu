@@ -28,6 +28,7 @@ int ensure_smem_attr(const void* func, int bytes);   // cbk_api.cu
 
 constexpr int kLgThreads = 512;
 constexpr int kLgCluster = 8;
+constexpr int kLgMaxVocab = kLgCluster * 56 * 1024;   // a segment's counts fit in shared memory
 constexpr uint32_t kLgPrompt = 0x80000000u;
 
 struct LogitsParams {
@@ -177,66 +178,62 @@ static int launch_logits(const LogitsParams& p, cudaStream_t st) {
 
 using namespace cbk;
 
-extern "C" int cbk_process_logits(const void* logits, int in_dtype, int64_t row_stride, int64_t rows, int64_t vocab,
-                                  const int64_t* history, int64_t history_stride, int64_t history_cap,
-                                  const int64_t* lengths, int64_t lengths_stride, const int64_t* n_prompt,
-                                  int64_t n_prompt_stride, float repetition, float presence, float frequency,
-                                  const float* bias, int64_t bias_stride, const int32_t* mask, int64_t mask_stride,
-                                  const int64_t* tree_tokens, const int32_t* tree_words, int64_t tree_stride,
-                                  int n_tree, void* out, int out_dtype, int64_t out_stride, int64_t* tokens,
-                                  int32_t* status, void* stream) {
-  if (in_dtype != CBK_BF16 && in_dtype != CBK_F16 && in_dtype != CBK_F32)
-    return set_error(CBK_ERR_UNSUPPORTED, "cbk_process_logits: dtype %d not supported", in_dtype);
-  if (out && out_dtype != in_dtype && out_dtype != CBK_F32)
+extern "C" int cbk_process_logits(const cbk_process_logits_args* a, void* stream) {
+  if (!a || a->size != sizeof(*a)) return set_error(CBK_ERR_INVALID, "cbk_process_logits: bad argument struct");
+  if (a->in_dtype != CBK_BF16 && a->in_dtype != CBK_F16 && a->in_dtype != CBK_F32)
+    return set_error(CBK_ERR_UNSUPPORTED, "cbk_process_logits: dtype %d not supported", a->in_dtype);
+  if (a->out && a->out_dtype != a->in_dtype && a->out_dtype != CBK_F32)
     return set_error(CBK_ERR_UNSUPPORTED, "cbk_process_logits: output dtype %d for input dtype %d (the same or fp32)",
-                     out_dtype, in_dtype);
-  if (vocab <= 0 || vocab > kLgCluster * 56 * 1024)
-    return set_error(CBK_ERR_UNSUPPORTED, "cbk_process_logits: vocabulary %lld (1 to %d)", (long long)vocab,
-                     kLgCluster * 56 * 1024);
-  if (rows < 0 || rows > (1 << 24)) return set_error(CBK_ERR_INVALID, "cbk_process_logits: %lld rows", (long long)rows);
-  if (rows == 0) return CBK_OK;
-  if (!logits || !tokens) return set_error(CBK_ERR_INVALID, "cbk_process_logits: null pointer argument");
-  if (!(repetition > 0.f)) return set_error(CBK_ERR_INVALID, "cbk_process_logits: repetition penalty must be > 0");
-  if (presence != presence || frequency != frequency)
+                     a->out_dtype, a->in_dtype);
+  if (a->vocab <= 0 || a->vocab > kLgMaxVocab)
+    return set_error(CBK_ERR_UNSUPPORTED, "cbk_process_logits: vocabulary %lld (1 to %d)", (long long)a->vocab,
+                     kLgMaxVocab);
+  if (a->rows < 0 || a->rows > (1 << 24))
+    return set_error(CBK_ERR_INVALID, "cbk_process_logits: %lld rows", (long long)a->rows);
+  if (a->rows == 0) return CBK_OK;
+  if (!a->logits || !a->tokens) return set_error(CBK_ERR_INVALID, "cbk_process_logits: null pointer argument");
+  if (!(a->repetition > 0.f)) return set_error(CBK_ERR_INVALID, "cbk_process_logits: repetition penalty must be > 0");
+  if (a->presence != a->presence || a->frequency != a->frequency)
     return set_error(CBK_ERR_INVALID, "cbk_process_logits: presence / frequency penalty is NaN");
-  if (row_stride < vocab || (out && out_stride < vocab) || (mask && mask_stride != 0 && mask_stride < (vocab + 31) / 32) ||
-      (bias && bias_stride != 0 && bias_stride < vocab))
+  if (a->row_stride < a->vocab || (a->out && a->out_stride < a->vocab) ||
+      (a->mask && a->mask_stride != 0 && a->mask_stride < (a->vocab + 31) / 32) ||
+      (a->bias && a->bias_stride != 0 && a->bias_stride < a->vocab))
     return set_error(CBK_ERR_INVALID, "cbk_process_logits: row stride shorter than a row");
-  if (history_cap < 0 || history_cap >= (int64_t{1} << 30) || n_tree < 0 || n_tree > 1024 ||
-      (n_tree > 0 && (!tree_tokens || !tree_words || tree_stride < (n_tree + 31) / 32)))
+  if (a->history_cap < 0 || a->history_cap >= (int64_t{1} << 30) || a->n_tree < 0 || a->n_tree > 1024 ||
+      (a->n_tree > 0 && (!a->tree_tokens || !a->tree_words || a->tree_stride < (a->n_tree + 31) / 32)))
     return set_error(CBK_ERR_INVALID, "cbk_process_logits: bad history or tree");
   LogitsParams p;
-  p.logits = logits;
-  p.out = out;
-  p.history = history_cap > 0 ? history : nullptr;
-  p.lengths = lengths;
-  p.n_prompt = n_prompt;
-  p.tree_tokens = tree_tokens;
-  p.mask = reinterpret_cast<const uint32_t*>(mask);
-  p.tree_words = reinterpret_cast<const uint32_t*>(tree_words);
-  p.bias = bias;
-  p.tokens = tokens;
-  p.status = status;
-  p.row_stride = row_stride;
-  p.out_stride = out_stride;
-  p.hist_stride = history_stride;
-  p.hist_cap = history_cap;
-  p.len_stride = lengths_stride;
-  p.prompt_stride = n_prompt_stride;
-  p.bias_stride = bias_stride;
-  p.mask_stride = mask_stride;
-  p.tree_stride = tree_stride;
-  p.rows = static_cast<int>(rows);
-  p.vocab = static_cast<int>(vocab);
-  p.seg = static_cast<int>((vocab + kLgCluster * 32 - 1) / (kLgCluster * 32) * 32);
-  p.n_tree = n_tree;
-  p.counted = p.history != nullptr || n_tree > 0;
-  p.repetition = repetition;
-  p.presence = presence;
-  p.frequency = frequency;
+  p.logits = a->logits;
+  p.out = a->out;
+  p.history = a->history_cap > 0 ? a->history : nullptr;
+  p.lengths = a->lengths;
+  p.n_prompt = a->n_prompt;
+  p.tree_tokens = a->tree_tokens;
+  p.mask = reinterpret_cast<const uint32_t*>(a->mask);
+  p.tree_words = reinterpret_cast<const uint32_t*>(a->tree_words);
+  p.bias = a->bias;
+  p.tokens = a->tokens;
+  p.status = a->status;
+  p.row_stride = a->row_stride;
+  p.out_stride = a->out_stride;
+  p.hist_stride = a->history_stride;
+  p.hist_cap = a->history_cap;
+  p.len_stride = a->lengths_stride;
+  p.prompt_stride = a->n_prompt_stride;
+  p.bias_stride = a->bias_stride;
+  p.mask_stride = a->mask_stride;
+  p.tree_stride = a->tree_stride;
+  p.rows = static_cast<int>(a->rows);
+  p.vocab = static_cast<int>(a->vocab);
+  p.seg = static_cast<int>((a->vocab + kLgCluster * 32 - 1) / (kLgCluster * 32) * 32);
+  p.n_tree = a->n_tree;
+  p.counted = p.history != nullptr || a->n_tree > 0;
+  p.repetition = a->repetition;
+  p.presence = a->presence;
+  p.frequency = a->frequency;
   auto st = static_cast<cudaStream_t>(stream);
-  const bool f32 = out && out_dtype == CBK_F32;
-  switch (in_dtype) {
+  const bool f32 = a->out && a->out_dtype == CBK_F32;
+  switch (a->in_dtype) {
     case CBK_F32: return launch_logits<CBK_F32, CBK_F32>(p, st);
     case CBK_BF16: return f32 ? launch_logits<CBK_BF16, CBK_F32>(p, st) : launch_logits<CBK_BF16, CBK_BF16>(p, st);
     default: return f32 ? launch_logits<CBK_F16, CBK_F32>(p, st) : launch_logits<CBK_F16, CBK_F16>(p, st);

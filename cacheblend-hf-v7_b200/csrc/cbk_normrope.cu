@@ -187,13 +187,9 @@ static int dispatch_norm_rope(NormRopeParams& p, int interleaved, int mode, cuda
 
 using namespace cbk;
 
-extern "C" int cbk_norm_rope_scatter(const void* q_src, int64_t q_row_stride, const void* k_src, int64_t k_row_stride,
-                                     const void* v_src, int64_t v_row_stride, const int64_t* positions,
-                                     const int64_t* rows, int64_t n, int n_q_heads, int n_kv_heads, int head_dim,
-                                     int rotary_dim, int interleaved, int dtype, const void* q_weight,
-                                     const void* k_weight, float eps, const void* rope_table, int64_t table_rows,
-                                     int rope_mode, void* q_out, void* k_cache, void* v_cache, int64_t kv_row_stride,
-                                     int64_t cap, int32_t* status, void* stream) {
+extern "C" int cbk_norm_rope_scatter(const cbk_norm_rope_scatter_args* a, void* stream) {
+  if (!a || a->size != sizeof(*a)) return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: bad argument struct");
+  const int dtype = a->dtype, head_dim = a->head_dim, rotary_dim = a->rotary_dim;
   if (dtype != CBK_BF16 && dtype != CBK_F16)
     return set_error(CBK_ERR_UNSUPPORTED, "cbk_norm_rope_scatter: dtype %d not supported", dtype);
   if (head_dim < 16 || head_dim > 256 || head_dim % 16 != 0)
@@ -201,54 +197,55 @@ extern "C" int cbk_norm_rope_scatter(const void* q_src, int64_t q_row_stride, co
   if (rotary_dim < 16 || rotary_dim > head_dim || rotary_dim % 16 != 0)
     return set_error(CBK_ERR_UNSUPPORTED, "cbk_norm_rope_scatter: rotary_dim %d (multiples of 16 up to head_dim %d)",
                      rotary_dim, head_dim);
-  if (rope_mode != CBK_ROPE_REF && rope_mode != CBK_ROPE_FP32)
-    return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: rope_mode %d", rope_mode);
-  if (n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads > 4096 || n_kv_heads > 4096)
-    return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: bad head counts %d / %d", n_q_heads, n_kv_heads);
-  if (n < 0 || cap < 0 || table_rows < 0)
+  if (a->rope_mode != CBK_ROPE_REF && a->rope_mode != CBK_ROPE_FP32)
+    return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: rope_mode %d", a->rope_mode);
+  if (a->n_q_heads <= 0 || a->n_kv_heads <= 0 || a->n_q_heads > 4096 || a->n_kv_heads > 4096)
+    return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: bad head counts %d / %d", a->n_q_heads, a->n_kv_heads);
+  if (a->n < 0 || a->cap < 0 || a->table_rows < 0)
     return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: negative size");
-  if (n == 0) return CBK_OK;
-  const int64_t qd = static_cast<int64_t>(n_q_heads) * head_dim, kd = static_cast<int64_t>(n_kv_heads) * head_dim;
-  if (!q_src || !k_src || !v_src || !positions || !rows || !rope_table || !q_out || !k_cache || !v_cache)
+  if (a->n == 0) return CBK_OK;
+  const int64_t qd = static_cast<int64_t>(a->n_q_heads) * head_dim, kd = static_cast<int64_t>(a->n_kv_heads) * head_dim;
+  if (!a->q_src || !a->k_src || !a->v_src || !a->positions || !a->rows || !a->rope_table || !a->q_out ||
+      !a->k_cache || !a->v_cache)
     return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: null pointer argument");
-  if ((q_weight == nullptr) != (k_weight == nullptr))
+  if ((a->q_weight == nullptr) != (a->k_weight == nullptr))
     return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: give both weights or neither");
-  if (q_row_stride < qd || k_row_stride < kd || v_row_stride < kd || kv_row_stride < kd || q_row_stride % 8 ||
-      k_row_stride % 8 || v_row_stride % 8 || kv_row_stride % 8)
+  if (a->q_row_stride < qd || a->k_row_stride < kd || a->v_row_stride < kd || a->kv_row_stride < kd ||
+      (a->q_row_stride | a->k_row_stride | a->v_row_stride | a->kv_row_stride) % 8)
     return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: row strides must cover a row and be multiples of 8");
-  const uintptr_t all = reinterpret_cast<uintptr_t>(q_src) | reinterpret_cast<uintptr_t>(k_src) |
-                        reinterpret_cast<uintptr_t>(v_src) | reinterpret_cast<uintptr_t>(q_weight) |
-                        reinterpret_cast<uintptr_t>(k_weight) | reinterpret_cast<uintptr_t>(rope_table) |
-                        reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_cache) |
-                        reinterpret_cast<uintptr_t>(v_cache);
+  const uintptr_t all = reinterpret_cast<uintptr_t>(a->q_src) | reinterpret_cast<uintptr_t>(a->k_src) |
+                        reinterpret_cast<uintptr_t>(a->v_src) | reinterpret_cast<uintptr_t>(a->q_weight) |
+                        reinterpret_cast<uintptr_t>(a->k_weight) | reinterpret_cast<uintptr_t>(a->rope_table) |
+                        reinterpret_cast<uintptr_t>(a->q_out) | reinterpret_cast<uintptr_t>(a->k_cache) |
+                        reinterpret_cast<uintptr_t>(a->v_cache);
   if (all & 15u) return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: pointers must be 16-byte aligned");
   NormRopeParams p;
-  p.q = static_cast<const uint16_t*>(q_src);
-  p.k = static_cast<const uint16_t*>(k_src);
-  p.v = static_cast<const uint16_t*>(v_src);
-  p.qw = static_cast<const uint16_t*>(q_weight);
-  p.kw = static_cast<const uint16_t*>(k_weight);
-  p.qs = q_row_stride;
-  p.ks = k_row_stride;
-  p.vs = v_row_stride;
-  p.pos = positions;
-  p.rows = rows;
-  p.table = static_cast<const float4*>(rope_table);
-  p.q_out = static_cast<uint16_t*>(q_out);
-  p.k_cache = static_cast<uint16_t*>(k_cache);
-  p.v_cache = static_cast<uint16_t*>(v_cache);
-  p.status = status;
-  p.n = n;
-  p.table_rows = table_rows;
-  p.cap = cap;
-  p.kv_stride = kv_row_stride;
-  p.n_q = n_q_heads;
-  p.n_kv = n_kv_heads;
+  p.q = static_cast<const uint16_t*>(a->q_src);
+  p.k = static_cast<const uint16_t*>(a->k_src);
+  p.v = static_cast<const uint16_t*>(a->v_src);
+  p.qw = static_cast<const uint16_t*>(a->q_weight);
+  p.kw = static_cast<const uint16_t*>(a->k_weight);
+  p.qs = a->q_row_stride;
+  p.ks = a->k_row_stride;
+  p.vs = a->v_row_stride;
+  p.pos = a->positions;
+  p.rows = a->rows;
+  p.table = static_cast<const float4*>(a->rope_table);
+  p.q_out = static_cast<uint16_t*>(a->q_out);
+  p.k_cache = static_cast<uint16_t*>(a->k_cache);
+  p.v_cache = static_cast<uint16_t*>(a->v_cache);
+  p.status = a->status;
+  p.n = a->n;
+  p.table_rows = a->table_rows;
+  p.cap = a->cap;
+  p.kv_stride = a->kv_row_stride;
+  p.n_q = a->n_q_heads;
+  p.n_kv = a->n_kv_heads;
   p.dim = head_dim;
   p.rotary = rotary_dim;
-  p.eps = eps;
+  p.eps = a->eps;
   p.inv_dim = 1.f / static_cast<float>(head_dim);
   auto st = static_cast<cudaStream_t>(stream);
-  return dtype == CBK_BF16 ? dispatch_norm_rope<CBK_BF16>(p, interleaved, rope_mode, st)
-                           : dispatch_norm_rope<CBK_F16>(p, interleaved, rope_mode, st);
+  return dtype == CBK_BF16 ? dispatch_norm_rope<CBK_BF16>(p, a->interleaved, a->rope_mode, st)
+                           : dispatch_norm_rope<CBK_F16>(p, a->interleaved, a->rope_mode, st);
 }

@@ -1,87 +1,631 @@
-// Attention of a tree of drafted tokens over the cache.
+// Attention of a tree of drafted tokens over the cache, on tcgen05 tensor cores.
 //
 // Node i of T nodes sees cache rows [0, n_ctx) and, of the rows n_ctx + j that
 // hold the nodes' own K and V, those whose bit j is set in words[i]:
 //   out[i][h] = softmax_t(scale q[i][h] . k[t][h / G]) . v[t][h / G].
 // n_ctx is read on the device, so a captured step stays valid as it advances.
 //
-// One CTA per (node, q head), a warp per key, an online softmax per warp and a
-// merge of the warps: every key row is read once per query row.
-#include "cbk_common.cuh"
+// The G q heads of a KV head share its keys, so the T * G query rows of a KV head
+// (row = node * G + head) are stacked into Q tiles of 128 rows, and the keys are
+// visited in tiles of 128.  The keys are split over CTAs -- grid (split, KV head,
+// pair of Q tiles), about one CTA per SM -- and tree_merge_kernel joins the
+// splits' (max, sum, O).  Up to 128 rows the call is bound by reading K and V
+// once; beyond, a CTA runs two Q tiles on the same K and V.
+//
+// A CTA holds two "slots", each with S / P (128 columns) and O (HD columns) in
+// TMEM and a softmax warpgroup of its own, so one slot's softmax runs while the
+// tensor core works for the other.  With two Q tiles, slot t is tile t and every
+// key tile goes to both; with one Q tile both slots hold that tile and take the
+// key tiles in turn, each with its own running max, sum and O (two partial
+// results for the merge).  Unit u of a CTA (slot u & 1) is then key tile u >> 1 or
+// u, and the MMA warp's order is the same for both: O += P(u) V(u), then
+// S(u + 2) = Q K(u + 2)^T, which overwrites P(u) after the PV that reads it.
+//
+// Warps (384 threads): 0 copies K and V tiles (TMA) into two rings; 1 issues the
+// MMAs; 2 holds TMEM; 2 and 3 clean the V tiles that reach past the context; 4..7
+// and 8..11 are the softmax of slots 0 and 1 (thread = row; a warp none of whose
+// 32 rows exists takes no part, so small trees cost little).
+//
+// Masked keys: their scores become -inf in registers and their weight is 0
+// exactly.  0 * NaN is NaN in an MMA, so rows behind the tree (whatever a cache
+// holds there) are zeroed in the V tile, and so is every non-finite element of
+// the tree's own V rows; the latter are added back on the CUDA cores, in the rows
+// that see them, by the epilogue (only when there are any).
+//
+// Rounding: S, the softmax statistics, O, the partial results and the merge are
+// fp32; P is rounded to the inputs' 16-bit type for the PV MMA (the tensor core
+// takes both operands in one type), the result once.
+// Every wait is bounded; on timeout the kernel sets CBK_STATUS_TIMEOUT, drains its
+// copies and MMAs, frees TMEM and returns.
+#include <algorithm>
+
+#include "cbk_attn_common.cuh"
 
 namespace cbk {
 
-constexpr int kTreeThreads = 128;
-constexpr int kTreeWarps = kTreeThreads / 32;
+int ensure_smem_attr(const void* func, int bytes);   // cbk_api.cu
 
-template <int DT, int HD>
-__global__ void __launch_bounds__(kTreeThreads)
-tree_attn_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
-                 int64_t kv_stride, const int64_t* __restrict__ n_ctx_ptr, const uint32_t* __restrict__ words,
-                 int64_t words_stride, int n_nodes, int64_t cap, int n_q, int group, float scale_log2,
-                 uint16_t* __restrict__ out, int32_t* status) {
-  using E = Elem<DT>;
-  constexpr int kD = HD / 32;
-  __shared__ float s_m[kTreeWarps], s_l[kTreeWarps], s_o[kTreeWarps][HD];
-  const int node = blockIdx.x, hq = blockIdx.y, h = hq / group;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t n_ctx = *n_ctx_ptr;
-  if (n_ctx < 0 || n_ctx + n_nodes > cap) {
-    if (threadIdx.x == 0 && node == 0 && hq == 0) report(status, CBK_STATUS_BAD_INDEX);
+constexpr int kTreeThreads = 384;
+constexpr int kTreeMaxNodes = 1024;
+constexpr uint32_t kTreeTmemCols = 512;
+constexpr int kTreeMergeWarps = 4;
+constexpr int kTreeMaxSplits = 160;          // at most one per SM
+
+struct TreeParams {
+  const uint16_t *q, *v;
+  const int64_t* n_ctx;
+  const uint32_t* words;
+  float* part_o;          // [slot][row_pitch][HD], relative to the slot's max
+  float2* part_ml;        // [slot][row_pitch] (running max in log2 units, row sum)
+  uint16_t* out;
+  int32_t* status;
+  int64_t kv_stride, words_stride, cap;
+  int n_nodes, n_q, group, rows, n_qt, n_pairs, n_splits, row_pitch;
+  float scale_log2;
+};
+
+// key tiles [j0, j1) of a split; tree-relative geometry of the call
+struct TreeSpan {
+  int64_t n_ctx, n_keys;
+  int n_tiles;
+  bool ok;
+};
+__device__ __forceinline__ TreeSpan tree_span(const TreeParams& p) {
+  TreeSpan s;
+  s.n_ctx = *p.n_ctx;
+  s.ok = s.n_ctx >= 0 && s.n_ctx <= p.cap - p.n_nodes;
+  s.n_keys = s.n_ctx + p.n_nodes;
+  s.n_tiles = static_cast<int>((s.n_keys + kBN - 1) / kBN);
+  return s;
+}
+__device__ __forceinline__ int split_start(int n_tiles, int n_splits, int s) {
+  return static_cast<int>(static_cast<int64_t>(n_tiles) * s / n_splits);
+}
+
+// 32 visibility bits of the keys at tree offsets [off, off + 32) of a node: offsets
+// below 0 are context, those from n on are behind the tree
+__device__ __forceinline__ uint32_t tree_bits(const uint32_t* w, int n, int off) {
+  if (off <= -32) return 0xffffffffu;
+  auto word = [&](int i) -> uint32_t {
+    if (i * 32 >= n) return 0u;
+    return n - i * 32 >= 32 ? w[i] : w[i] & ((1u << (n - i * 32)) - 1u);
+  };
+  if (off < 0) return ((1u << -off) - 1u) | (word(0) << -off);
+  return __funnelshift_r(word(off >> 5), word((off >> 5) + 1), off & 31);
+}
+
+template <int HD, int NQ, int NST>
+struct TreeSmem {
+  static constexpr int kQBytes = kBM * HD * 2;
+  static constexpr int kKVBytes = kBN * HD * 2;
+  static constexpr int kK0 = NQ * kQBytes;
+  static constexpr int kV0 = kK0 + NST * kKVBytes;
+  static constexpr int kBar = kV0 + NST * kKVBytes;
+  static constexpr int kBars = 5 * NST + 9;
+  static constexpr int kMisc = kBar + kBars * 8;       // tmem slot, abort flag, non-finite flag
+  static constexpr int kTotal = kMisc + 16;
+  // more than half an SM's shared memory: one CTA (holding all 512 TMEM columns) per SM
+  static constexpr int kAlloc = (kTotal + 1024) > 122880 ? (kTotal + 1024) : 122880;
+};
+
+template <int DT, int HD, int NQ, int NST>
+__global__ void __launch_bounds__(kTreeThreads, 1)
+tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                 const TreeParams p) {
+  using L = TreeSmem<HD, NQ, NST>;
+  enum { KFULL = 0, KEMPTY = NST, VFULL = 2 * NST, VEMPTY = 3 * NST, VCLEAN = 4 * NST, SFULL = 5 * NST,
+         PHALF = SFULL + 2, PFULL = SFULL + 4, ODONE = SFULL + 6, DRAIN = SFULL + 8 };
+  const int split = blockIdx.x, kvh = blockIdx.y, pair = blockIdx.z;
+  const TreeSpan sp = tree_span(p);
+  if (!sp.ok) {
+    if (threadIdx.x == 0 && split == 0 && kvh == 0 && pair == 0) report(p.status, CBK_STATUS_BAD_INDEX);
     return;
   }
-  float qf[kD], o[kD], m = -INFINITY, l = 0.f;
+  const int j0 = split_start(sp.n_tiles, p.n_splits, split);
+  const int n = split_start(sp.n_tiles, p.n_splits, split + 1) - j0;      // key tiles of this CTA
+  if (n == 0) return;
+  const bool two = NQ == 2 && 2 * pair + 1 < p.n_qt;       // two Q tiles, else one in both slots
+  const int n_units = two ? 2 * n : n;
+  // first local key tile that is not all context
+  const int n_full = static_cast<int>(sp.n_ctx / kBN);
+  const int m0 = n_full > j0 ? min(n_full - j0, n) : 0;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* sbase = smem_raw + (base - raw_addr);
+  const uint32_t sK0 = base + L::kK0, sV0 = base + L::kV0;
+  auto bar = [&](int i) { return base + L::kBar + 8u * i; };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sbase + L::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sbase + L::kMisc + 4);
+  volatile int* odd_flag = reinterpret_cast<volatile int*>(sbase + L::kMisc + 8);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  bool failed = false;
+  auto wait_all = [&](uint32_t b, uint32_t parity) {
+    return __all_sync(0xffffffffu, wait_or_abort(b, parity, abort_flag));
+  };
+  auto tile_rows = [&](int t) {                  // existing rows of slot t's Q tile
+    return min(kBM, p.rows - (2 * pair + (two ? t : 0)) * kBM);
+  };
+  auto load_tile = [&](const CUtensorMap* tm, uint32_t dst, uint32_t b, int g) {
+    mbar_expect_tx(b, L::kKVBytes);
 #pragma unroll
-  for (int d = 0; d < kD; ++d) {
-    qf[d] = E::to_f(q[(static_cast<int64_t>(node) * n_q + hq) * HD + lane * kD + d]);
-    o[d] = 0.f;
-  }
-  for (int64_t t = warp; t < n_ctx + n_nodes; t += kTreeWarps) {
-    if (t >= n_ctx) {
-      const int j = static_cast<int>(t - n_ctx);
-      if (!((words[node * words_stride + j / 32] >> (j % 32)) & 1u)) continue;
-    }
-    const uint16_t* kr = kc + t * kv_stride + static_cast<int64_t>(h) * HD + lane * kD;
-    const uint16_t* vr = vc + t * kv_stride + static_cast<int64_t>(h) * HD + lane * kD;
-    float s = 0.f;
+    for (int h = 0; h < HD / 64; ++h) tma_load_3d(dst + h * (kBN * 128), tm, b, h * 64, kvh, (j0 + g) * kBN);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
 #pragma unroll
-    for (int d = 0; d < kD; ++d) s = fmaf(qf[d], E::to_f(kr[d]), s);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= scale_log2;
-    const float m_new = fmaxf(m, s);
-    const float a = m == m_new ? 1.f : ex2(m - m_new), w = ex2(s - m_new);
-    l = l * a + w;
-    m = m_new;
-#pragma unroll
-    for (int d = 0; d < kD; ++d) o[d] = fmaf(w, E::to_f(vr[d]), o[d] * a);
-  }
-  if (lane == 0) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-  }
-#pragma unroll
-  for (int d = 0; d < kD; ++d) s_o[warp][lane * kD + d] = o[d];
-  __syncthreads();
-  for (int d = threadIdx.x; d < HD; d += kTreeThreads) {
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-    for (int w = 0; w < kTreeWarps; ++w)
-      if (s_l[w] != 0.f) M = fmaxf(M, s_m[w]);
-    for (int w = 0; w < kTreeWarps; ++w)
-      if (s_l[w] != 0.f) {
-        const float wt = ex2(s_m[w] - M);
-        L += wt * s_l[w];
-        acc += wt * s_o[w][d];
+      for (int i = 0; i < NST; ++i) {
+        mbar_init(bar(KFULL + i), 1);
+        mbar_init(bar(KEMPTY + i), 1);
+        mbar_init(bar(VFULL + i), 1);
+        mbar_init(bar(VEMPTY + i), 3);           // the MMAs' commit and the two cleaning warps
+        mbar_init(bar(VCLEAN + i), 2);
       }
-    out[(static_cast<int64_t>(node) * n_q + hq) * HD + d] = E::from_f(L == 0.f ? 0.f : acc / L);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int active = (tile_rows(t) + 31) / 32;
+        mbar_init(bar(SFULL + t), 1);
+        mbar_init(bar(PHALF + t), active);
+        mbar_init(bar(PFULL + t), active);
+        mbar_init(bar(ODONE + t), 1);
+      }
+      mbar_init(bar(DRAIN), 1);
+      *abort_flag = 0;
+      *odd_flag = 0;
+      fence_barrier_init();
+    }
+    __syncwarp();
+    if (elect_one()) {                           // the first tiles are on their way before the rest is set up
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+      for (int g = 0; g < min(n, NST); ++g) {
+        load_tile(&tm_k, sK0 + g * L::kKVBytes, bar(KFULL + g), g);
+        load_tile(&tm_v, sV0 + g * L::kKVBytes, bar(VFULL + g), g);
+      }
+    }
+  } else if (warp == 2) {
+    tmem_alloc(smem_u32(tmem_slot), kTreeTmemCols);
+    tmem_relinquish();
+  } else if (warp >= 4) {
+    // Q tiles in the layout a 128-byte-swizzled TMA copy leaves: 16-byte piece c of
+    // row r at piece c ^ (r & 7); rows that do not exist are zero
+    constexpr int kVec = HD / 8;
+    const int n_q_tiles = two ? 2 : 1;
+    for (int i = threadIdx.x - 128; i < n_q_tiles * kBM * kVec; i += kTreeThreads - 128) {
+      const int r = i / kVec, c = i % kVec;
+      const int row = 2 * pair * kBM + r;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (row < p.rows)
+        x = ld_vec(p.q + (static_cast<int64_t>(row / p.group) * p.n_q + kvh * p.group + row % p.group) * HD + c * 8);
+      *reinterpret_cast<uint4*>(sbase + (r / kBM) * L::kQBytes + (c >> 3) * (kBM * 128) + (r % kBM) * 128 +
+                                ((c ^ r) & 7) * 16) = x;
+    }
+    fence_proxy_async_smem();
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // the merge kernel (a programmatic dependent) may be placed as SMs free up
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    const bool leader = elect_one();
+    int last_k = min(n, NST) - 1, last_v = last_k;      // last tiles issued
+    for (int g = NST; g < n; ++g) {
+      const int st = g % NST;
+      const uint32_t par = (g / NST - 1) & 1;
+      if (!wait_all(bar(KEMPTY + st), par)) {
+        failed = true;
+        break;
+      }
+      if (leader) load_tile(&tm_k, sK0 + st * L::kKVBytes, bar(KFULL + st), g);
+      last_k = g;
+      if (!wait_all(bar(VEMPTY + st), par)) {
+        failed = true;
+        break;
+      }
+      if (leader) load_tile(&tm_v, sV0 + st * L::kKVBytes, bar(VFULL + st), g);
+      last_v = g;
+    }
+    // drain: every armed copy must land before the CTA can retire
+    for (int g = max(0, last_k - NST + 1); g <= last_k; ++g)
+      if (!__all_sync(0xffffffffu, mbar_wait(bar(KFULL + g % NST), (g / NST) & 1))) failed = true;
+    for (int g = max(0, last_v - NST + 1); g <= last_v; ++g)
+      if (!__all_sync(0xffffffffu, mbar_wait(bar(VFULL + g % NST), (g / NST) & 1))) failed = true;
+  } else if (warp == 1) {
+    // ------------------------------------------------------------- MMA issuer
+    const bool leader = elect_one();
+    const uint32_t idesc_s = umma_idesc_f16(DT, kBM, kBN, 0);
+    const uint32_t idesc_o = umma_idesc_f16(DT, kBM, HD, 1);
+    const uint64_t dq0 = umma_desc_sw128(base, 16, 1024);
+    const uint64_t dk0 = umma_desc_sw128(sK0, 16, 1024);
+    const uint64_t dv0 = umma_desc_sw128(sV0, kBN * 128, 1024);
+    auto unit_tile = [&](int u) { return two ? u >> 1 : u; };
+    // S of unit u, waiting for its K tile at the tile's first use and releasing it after its last
+    auto issue_s = [&](int u) -> bool {
+      const int t = u & 1, g = unit_tile(u), st = g % NST;
+      if (!(two && t == 1) && !wait_all(bar(KFULL + st), (g / NST) & 1)) return false;
+      tc_fence_after();
+      const uint64_t q0 = dq0 + ((two && t) ? (L::kQBytes >> 4) : 0);
+      const uint64_t k0 = dk0 + ((st * L::kKVBytes) >> 4);
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        const uint32_t off = ((kk >> 2) * (kBM * 128) + (kk & 3) * 32) >> 4;
+        if (leader) umma_f16_ss(tmem + 256 * t, q0 + off, k0 + off, idesc_s, kk > 0 ? 1u : 0u);
+      }
+      if (leader) {
+        umma_commit(bar(SFULL + t));
+        if (!two || t == 1) umma_commit(bar(KEMPTY + st));
+      }
+      return true;
+    };
+    auto issue_pv = [&](int t, int st, bool acc, int kk_lo, int kk_hi) {
+      const uint64_t v0 = dv0 + ((st * L::kKVBytes) >> 4);
+#pragma unroll
+      for (int kk = kk_lo; kk < kk_hi; ++kk)
+        if (leader)
+          umma_f16_ts(tmem + 256 * t + kBN, tmem + 256 * t + kk * 8, v0 + ((kk * 16 * 128) >> 4), idesc_o,
+                      (acc || kk > 0) ? 1u : 0u);
+    };
+    for (int u = 0; u < min(n_units, 2) && !failed; ++u)
+      if (!issue_s(u)) failed = true;
+    for (int u = 0; u < n_units && !failed; ++u) {
+      const int t = u & 1, g = unit_tile(u), st = g % NST, k = u >> 1;     // unit k of its slot
+      if (!(two && t == 1)) {
+        const bool ok = g < m0 ? wait_all(bar(VFULL + st), (g / NST) & 1)
+                               : wait_all(bar(VCLEAN + st), ((g - m0) / NST) & 1);
+        if (!ok) {
+          failed = true;
+          break;
+        }
+      }
+      if (!wait_all(bar(PHALF + t), k & 1)) {
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      issue_pv(t, st, k > 0, 0, kBN / 32);
+      if (!wait_all(bar(PFULL + t), k & 1)) {
+        failed = true;
+        break;
+      }
+      tc_fence_after();
+      issue_pv(t, st, true, kBN / 32, kBN / 16);
+      if (leader && (!two || t == 1)) umma_commit(bar(VEMPTY + st));
+      if (u + 2 < n_units) {
+        if (!issue_s(u + 2)) failed = true;
+      } else if (leader) {
+        umma_commit(bar(ODONE + t));
+      }
+    }
+    // drain: all MMAs issued by this warp complete before TMEM is released
+    if (leader) umma_commit(bar(DRAIN));
+    if (!__all_sync(0xffffffffu, mbar_wait(bar(DRAIN), 0))) failed = true;
+  } else if (warp < 4) {
+    // -------------------------------------- V tiles that reach past the context
+    constexpr uint32_t kExp = DT == CBK_BF16 ? 0x7f80u : 0x7c00u;
+    // Tiles of context pass through: these warps see every phase of every stage, and a
+    // stage is filled again only once they have left it.
+    for (int g = 0; g < n; ++g) {
+      const int st = g % NST;
+      if (!wait_all(bar(VFULL + st), (g / NST) & 1)) {
+        failed = true;
+        break;
+      }
+      if (g < m0) {
+        if (lane == 0) mbar_arrive(bar(VEMPTY + st));
+        continue;
+      }
+      const int64_t t0 = static_cast<int64_t>(j0 + g) * kBN;
+      const int tree0 = static_cast<int>(sp.n_ctx > t0 ? sp.n_ctx - t0 : 0);                  // first row of the tree
+      const int end = static_cast<int>(min(static_cast<int64_t>(kBN), sp.n_keys - t0));       // first row behind it
+      uint4* tile = reinterpret_cast<uint4*>(sbase + L::kV0 + st * L::kKVBytes);
+      bool odd = false;
+      for (int i = threadIdx.x - 64; i < L::kKVBytes / 16; i += 64) {
+        const int r = (i >> 3) % kBN;
+        if (r < tree0) continue;
+        uint4 x = tile[i];
+        uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+        if (r >= end) {
+          tile[i] = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+        bool here = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((w[e] & kExp) == kExp) w[e] &= 0xffff0000u, here = true;
+          if ((w[e] & (kExp << 16)) == (kExp << 16)) w[e] &= 0x0000ffffu, here = true;
+        }
+        if (here) {
+          tile[i] = x;
+          odd = true;
+        }
+      }
+      if (odd) *odd_flag = 1;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(VCLEAN + st));
+        mbar_arrive(bar(VEMPTY + st));
+      }
+    }
+  } else {
+    // ----------------------------------------------- softmax + epilogue warps
+    const int t = (warp - 4) >> 2, sub = warp & 3;
+    const int row = sub * 32 + lane;                        // row of the Q tile
+    const int n_rows = tile_rows(t);
+    const int n_t = two ? n : (n - t + 1) / 2;              // units of this slot
+    if (sub * 32 < n_rows && n_t > 0) {
+      const uint32_t lane_off = static_cast<uint32_t>(sub * 32) << 16;
+      const uint32_t tS = tmem + 256 * t + lane_off, tO = tS + kBN;
+      const float sl2 = p.scale_log2;
+      const int node = min((2 * pair + (two ? t : 0)) * kBM + row, p.rows - 1) / p.group;
+      const uint32_t* words = p.words + node * p.words_stride;
+      float m_used = -INFINITY, l_sum = 0.f;
+      for (int k = 0; k < n_t; ++k) {
+        const int g = two ? k : 2 * k + t;
+        if (!wait_all(bar(SFULL + t), k & 1)) {
+          failed = true;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[kBN];
+#pragma unroll
+        for (int c4 = 0; c4 < kBN / 32; ++c4) tmem_ld32(tS + c4 * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c4 * 32]));
+        tmem_wait_ld();
+        const bool masked = g >= m0;
+        if (masked) {
+          const int off = static_cast<int>(static_cast<int64_t>(j0 + g) * kBN - sp.n_ctx);
+#pragma unroll
+          for (int c4 = 0; c4 < kBN / 32; ++c4) {
+            const uint32_t bits = tree_bits(words, p.n_nodes, off + 32 * c4);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[c4 * 32 + e] = (bits >> e) & 1u ? s[c4 * 32 + e] : 0xff800000u;
+          }
+        }
+        float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kBN; c += 8) {
+          x0 = max3f(x0, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+          x1 = max3f(x1, __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
+          x2 = max3f(x2, __uint_as_float(s[c + 4]), __uint_as_float(s[c + 5]));
+          x3 = max3f(x3, __uint_as_float(s[c + 6]), __uint_as_float(s[c + 7]));
+        }
+        const float m_tile = max3f(x0, x1, fmaxf(x2, x3)) * sl2;
+        float alpha = 1.f;
+        bool rescale = false;
+        if (k == 0) {
+          m_used = m_tile;
+        } else if (m_tile > m_used + 8.f) {      // P stays below 2^8 under the older max
+          alpha = ex2(m_used - m_tile);
+          m_used = m_tile;
+          rescale = true;
+        }
+        float ra0 = 0.f, ra1 = 0.f, rb0 = 0.f, rb1 = 0.f;
+        // no visible key so far: a finite offset keeps the masked arguments at -inf
+        const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+#pragma unroll
+        for (int c4 = 0; c4 < kBN / 32; ++c4) {
+          uint32_t pk[16];
+          if (masked) exp_chunk<DT, 0>(s, c4, sl2, neg_m, ra0, ra1, rb0, rb1, pk);
+          else exp_chunk<DT>(s, c4, sl2, neg_m, ra0, ra1, rb0, rb1, pk);
+          tmem_st16(tS + c4 * 16, pk);
+          if (c4 == kBN / 64 - 1) {
+            // keys 0-63 of P stored: their PV may start, once O has the new max (O is
+            // stable: the commit behind this tile's S covered the PV before it)
+            if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+              for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(tO + c * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st32(tO + c * 32, o);
+              }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(PHALF + t));
+          }
+        }
+        l_sum = l_sum * alpha + (ra0 + ra1) + (rb0 + rb1);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(PFULL + t));
+      }
+      if (!failed && !wait_all(bar(ODONE + t), 0)) failed = true;
+      if (!failed) {
+        tc_fence_after();
+        const int64_t slot = ((static_cast<int64_t>(kvh) * p.n_pairs + pair) * p.n_splits + split) * 2 + t;
+        float* po = p.part_o + (slot * p.row_pitch + row) * HD;
+        const bool fix = *odd_flag != 0;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + c * 32, o);
+          tmem_wait_ld();
+          if (row < n_rows && fix) {
+            // non-finite elements of the V rows this row sees in this slot's key tiles
+            for (int g = max(m0, two ? 0 : t); g < n; ++g) {
+              if (!two && ((g ^ t) & 1)) continue;
+              const int off = static_cast<int>(static_cast<int64_t>(j0 + g) * kBN - sp.n_ctx);
+              for (int b = max(0, -off); b < kBN && off + b < p.n_nodes; ++b) {
+                const int j = off + b;
+                if (!((words[j >> 5] >> (j & 31)) & 1u)) continue;
+                const uint16_t* vr = p.v + (sp.n_ctx + j) * p.kv_stride + static_cast<int64_t>(kvh) * HD + c * 32;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float x = Elem<DT>::to_f(vr[e]);
+                  if (!(fabsf(x) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+                }
+              }
+            }
+          }
+          if (row < n_rows) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                           :: "l"(po + c * 32 + 8 * h), "r"(o[8 * h]), "r"(o[8 * h + 1]), "r"(o[8 * h + 2]),
+                              "r"(o[8 * h + 3]), "r"(o[8 * h + 4]), "r"(o[8 * h + 5]), "r"(o[8 * h + 6]),
+                              "r"(o[8 * h + 7]) : "memory");
+          }
+          __syncwarp();
+        }
+        if (row < n_rows) p.part_ml[slot * p.row_pitch + row] = make_float2(m_used, l_sum);
+      }
+    }
+  }
+
+  if (failed) {
+    *abort_flag = 1;
+    report(p.status, CBK_STATUS_TIMEOUT);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTreeTmemCols);
+  }
+}
+
+// Merge of the splits, a warp per query row: O = sum_i w_i O_i / sum_i w_i l_i,
+// w_i = 2^(m_i - M) over the row's slots that hold a key tile, in their order.  A
+// row that sees nothing has every l_i = 0 and gets zeros.
+template <int DT, int HD>
+__global__ void __launch_bounds__(kTreeMergeWarps * 32)
+tree_merge_kernel(const TreeParams p, int n_kv) {
+  using E = Elem<DT>;
+  constexpr int kD = HD / 32;
+  __shared__ float s_w[kTreeMergeWarps][2 * kTreeMaxSplits];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t gr = static_cast<int64_t>(blockIdx.x) * kTreeMergeWarps + warp;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (gr >= static_cast<int64_t>(n_kv) * p.rows) return;
+  const TreeSpan sp = tree_span(p);
+  if (!sp.ok) return;                                  // reported by the attention kernel
+  const int kvh = static_cast<int>(gr / p.rows), row = static_cast<int>(gr % p.rows);
+  const int qt = row / kBM, pair = qt / 2, r = row % kBM;
+  const bool two = (qt | 1) < p.n_qt;
+  // slot of index i: split i with the row's tile, or split i / 2 with half i & 1 of its key tiles
+  const int n_i = two ? p.n_splits : 2 * p.n_splits;
+  const int64_t slot0 = (static_cast<int64_t>(kvh) * p.n_pairs + pair) * p.n_splits * 2;
+  auto slot_of = [&](int i) { return two ? slot0 + 2 * i + (qt & 1) : slot0 + i; };
+  auto holds = [&](int i) {
+    const int s = two ? i : i >> 1;
+    return split_start(sp.n_tiles, p.n_splits, s + 1) - split_start(sp.n_tiles, p.n_splits, s) > (two ? 0 : (i & 1));
+  };
+  float M = -INFINITY;
+  for (int i = lane; i < n_i; i += 32) {
+    const float2 ml = holds(i) ? p.part_ml[slot_of(i) * p.row_pitch + r] : make_float2(-INFINITY, 0.f);
+    if (ml.y != 0.f) M = fmaxf(M, ml.x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float lsum = 0.f;
+  for (int i = lane; i < n_i; i += 32) {
+    const float2 ml = holds(i) ? p.part_ml[slot_of(i) * p.row_pitch + r] : make_float2(-INFINITY, 0.f);
+    const float w = ml.y != 0.f ? ex2(ml.x - M) : 0.f;
+    s_w[warp][i] = holds(i) ? w : -1.f;
+    lsum += ml.y != 0.f ? w * ml.y : 0.f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
+  __syncwarp();
+  float acc[kD];
+#pragma unroll
+  for (int d = 0; d < kD; ++d) acc[d] = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < n_i; ++i) {
+    const float w = s_w[warp][i];
+    if (w < 0.f) continue;                             // nothing was written there
+    const float* po = p.part_o + (slot_of(i) * p.row_pitch + r) * HD + lane * kD;
+    if constexpr (kD == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(po);
+      acc[0] = fmaf(w, x.x, acc[0]);
+      acc[1] = fmaf(w, x.y, acc[1]);
+      acc[2] = fmaf(w, x.z, acc[2]);
+      acc[3] = fmaf(w, x.w, acc[3]);
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(po);
+      acc[0] = fmaf(w, x.x, acc[0]);
+      acc[1] = fmaf(w, x.y, acc[1]);
+    }
+  }
+  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+  uint16_t* o = p.out + (static_cast<int64_t>(row / p.group) * p.n_q + kvh * p.group + row % p.group) * HD + lane * kD;
+#pragma unroll
+  for (int d = 0; d < kD; d += 2) *reinterpret_cast<uint32_t*>(o + d) = Pk<DT>::cvt(acc[d] * inv, acc[d + 1] * inv);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct TreeLayout {
+  int rows, n_qt, n_pairs, n_splits, row_pitch;
+  size_t off_o, bytes;
+};
+
+static TreeLayout tree_layout(int n_nodes, int64_t cap, int n_q_heads, int n_kv_heads, int head_dim) {
+  TreeLayout t;
+  t.rows = n_nodes * (n_q_heads / n_kv_heads);
+  t.n_qt = (t.rows + kBM - 1) / kBM;
+  t.n_pairs = (t.n_qt + 1) / 2;
+  const int64_t units = static_cast<int64_t>(n_kv_heads) * t.n_pairs;
+  const int64_t sms = std::min(attn_sm_count(), kTreeMaxSplits);
+  t.n_splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / units, (cap + kBN - 1) / kBN)));
+  t.row_pitch = (std::min(t.rows, kBM) + 7) / 8 * 8;
+  const size_t slots = static_cast<size_t>(units) * t.n_splits * 2;
+  t.off_o = (slots * t.row_pitch * sizeof(float2) + 255) & ~static_cast<size_t>(255);
+  t.bytes = t.off_o + slots * t.row_pitch * head_dim * sizeof(float);
+  return t;
+}
+
+template <int DT, int HD, int NQ, int NST>
+static int launch_tree(const cbk_tree_attn_args* a, const TreeParams& p, cudaStream_t st) {
+  CUtensorMap mk, mv;
+  if (int rc = attn_make_map(&mk, a->k_cache, DT, HD, a->n_kv_heads, a->cap, a->kv_row_stride, 1, kBN)) return rc;
+  if (int rc = attn_make_map(&mv, a->v_cache, DT, HD, a->n_kv_heads, a->cap, a->kv_row_stride, 1, kBN)) return rc;
+  auto kern = tree_attn_kernel<DT, HD, NQ, NST>;
+  constexpr int smem = TreeSmem<HD, NQ, NST>::kAlloc;
+  static_assert(smem <= 227 * 1024, "shared memory of tree_attn_kernel");
+  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem)) return rc;
+  kern<<<dim3(p.n_splits, a->n_kv_heads, p.n_pairs), kTreeThreads, smem, st>>>(mk, mv, p);
+  if (int rc = check_launch("tree_attn_kernel")) return rc;
+  cudaLaunchConfig_t cfg = {};
+  const int64_t rows = static_cast<int64_t>(a->n_kv_heads) * p.rows;
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + kTreeMergeWarps - 1) / kTreeMergeWarps));
+  cfg.blockDim = dim3(kTreeMergeWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_merge_kernel<DT, HD>, p, static_cast<int>(a->n_kv_heads));
+  if (e != cudaSuccess) return set_error(CBK_ERR_CUDA, "tree_merge_kernel launch: %s", cudaGetErrorString(e));
+  return check_launch("tree_merge_kernel");
+}
+
+template <int DT>
+static int dispatch_tree(const cbk_tree_attn_args* a, const TreeParams& p, cudaStream_t st) {
+  // one Q tile: a deeper ring (the call is bound by reading K and V); two: their
+  // second tile takes a stage's room
+  if (a->head_dim == 128)
+    return p.n_qt == 1 ? launch_tree<DT, 128, 1, 3>(a, p, st) : launch_tree<DT, 128, 2, 2>(a, p, st);
+  return p.n_qt == 1 ? launch_tree<DT, 64, 1, 6>(a, p, st) : launch_tree<DT, 64, 2, 5>(a, p, st);
 }
 
 }  // namespace cbk
 
 using namespace cbk;
-
-constexpr int kTreeMaxNodes = 1024;
 
 static int check_tree_geometry(const char* who, int n_nodes, int64_t cap, int n_q_heads, int n_kv_heads,
                                int head_dim) {
@@ -100,42 +644,57 @@ extern "C" size_t cbk_tree_attn_workspace_bytes(int n_nodes, int64_t cap, int n_
                                                 int head_dim) {
   if (check_tree_geometry("cbk_tree_attn_workspace_bytes", n_nodes, cap, n_q_heads, n_kv_heads, head_dim) != CBK_OK)
     return 0;
-  return 256;
+  return tree_layout(std::max(n_nodes, 1), std::max<int64_t>(cap, 1), n_q_heads, n_kv_heads, head_dim).bytes;
 }
 
-extern "C" int cbk_tree_attn(const void* q, const void* k_cache, const void* v_cache, int64_t kv_row_stride,
-                             const int64_t* n_ctx, const int32_t* words, int64_t words_stride, int n_nodes,
-                             int64_t cap, int n_q_heads, int n_kv_heads, int head_dim, float scale, int dtype,
-                             void* out, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
-  if (dtype != CBK_BF16 && dtype != CBK_F16)
-    return set_error(CBK_ERR_UNSUPPORTED, "cbk_tree_attn: dtype %d not supported", dtype);
-  if (int rc = check_tree_geometry("cbk_tree_attn", n_nodes, cap, n_q_heads, n_kv_heads, head_dim)) return rc;
-  if (n_nodes == 0) return CBK_OK;
-  if (kv_row_stride < static_cast<int64_t>(n_kv_heads) * head_dim || kv_row_stride % 8 != 0 ||
-      words_stride < (n_nodes + 31) / 32)
-    return set_error(CBK_ERR_INVALID, "cbk_tree_attn: bad strides (cache %lld, words %lld)", (long long)kv_row_stride,
-                     (long long)words_stride);
-  if (!q || !k_cache || !v_cache || !n_ctx || !words || !out || !workspace)
+extern "C" int cbk_tree_attn(const cbk_tree_attn_args* a, void* stream) {
+  if (!a || a->size != sizeof(*a)) return set_error(CBK_ERR_INVALID, "cbk_tree_attn: bad argument struct");
+  if (a->dtype != CBK_BF16 && a->dtype != CBK_F16)
+    return set_error(CBK_ERR_UNSUPPORTED, "cbk_tree_attn: dtype %d not supported", a->dtype);
+  if (int rc = check_tree_geometry("cbk_tree_attn", a->n_nodes, a->cap, a->n_q_heads, a->n_kv_heads, a->head_dim))
+    return rc;
+  if (a->n_nodes == 0) return CBK_OK;
+  if (a->kv_row_stride < static_cast<int64_t>(a->n_kv_heads) * a->head_dim || a->kv_row_stride % 8 != 0 ||
+      a->words_stride < (a->n_nodes + 31) / 32)
+    return set_error(CBK_ERR_INVALID, "cbk_tree_attn: bad strides (cache %lld, words %lld)",
+                     (long long)a->kv_row_stride, (long long)a->words_stride);
+  if (!a->q || !a->k_cache || !a->v_cache || !a->n_ctx || !a->words || !a->out || !a->workspace)
     return set_error(CBK_ERR_INVALID, "cbk_tree_attn: null pointer argument");
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
-       reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15u)
-    return set_error(CBK_ERR_INVALID, "cbk_tree_attn: q, caches, out and workspace must be 16-byte aligned");
-  const size_t need = cbk_tree_attn_workspace_bytes(n_nodes, cap, n_q_heads, n_kv_heads, head_dim);
-  if (workspace_bytes < need)
-    return set_error(CBK_ERR_WORKSPACE, "cbk_tree_attn: workspace %zu < %zu bytes", workspace_bytes, need);
-  const dim3 grid(n_nodes, n_q_heads);
+  if (reinterpret_cast<uintptr_t>(a->workspace) & 31u)
+    return set_error(CBK_ERR_INVALID, "cbk_tree_attn: the workspace must be 32-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k_cache) |
+       reinterpret_cast<uintptr_t>(a->v_cache) | reinterpret_cast<uintptr_t>(a->out)) & 15u)
+    return set_error(CBK_ERR_INVALID, "cbk_tree_attn: q, caches and out must be 16-byte aligned");
+  if (!(a->scale > 0.f) || !(a->scale < INFINITY))
+    return set_error(CBK_ERR_INVALID, "cbk_tree_attn: scale must be positive and finite");
+  const TreeLayout lay = tree_layout(a->n_nodes, a->cap, a->n_q_heads, a->n_kv_heads, a->head_dim);
+  if (lay.n_pairs > 65535 || a->n_kv_heads > 65535)
+    return set_error(CBK_ERR_UNSUPPORTED, "cbk_tree_attn: too many query rows");
+  if (a->workspace_bytes < 0 || static_cast<size_t>(a->workspace_bytes) < lay.bytes)
+    return set_error(CBK_ERR_WORKSPACE, "cbk_tree_attn: workspace %lld < %zu bytes", (long long)a->workspace_bytes,
+                     lay.bytes);
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  TreeParams p;
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.v = static_cast<const uint16_t*>(a->v_cache);
+  p.n_ctx = a->n_ctx;
+  p.words = reinterpret_cast<const uint32_t*>(a->words);
+  p.part_ml = reinterpret_cast<float2*>(ws);
+  p.part_o = reinterpret_cast<float*>(ws + lay.off_o);
+  p.out = static_cast<uint16_t*>(a->out);
+  p.status = a->status;
+  p.kv_stride = a->kv_row_stride;
+  p.words_stride = a->words_stride;
+  p.cap = a->cap;
+  p.n_nodes = a->n_nodes;
+  p.n_q = a->n_q_heads;
+  p.group = a->n_q_heads / a->n_kv_heads;
+  p.rows = lay.rows;
+  p.n_qt = lay.n_qt;
+  p.n_pairs = lay.n_pairs;
+  p.n_splits = lay.n_splits;
+  p.row_pitch = lay.row_pitch;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
   auto st = static_cast<cudaStream_t>(stream);
-  const float sl2 = scale * 1.4426950408889634f;
-#define CBK_TREE(DT, HD)                                                                                           \
-  tree_attn_kernel<DT, HD><<<grid, kTreeThreads, 0, st>>>(                                                         \
-      static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache), static_cast<const uint16_t*>(v_cache), \
-      kv_row_stride, n_ctx, reinterpret_cast<const uint32_t*>(words), words_stride, n_nodes, cap, n_q_heads,       \
-      n_q_heads / n_kv_heads, sl2, static_cast<uint16_t*>(out), status)
-  if (dtype == CBK_BF16) {
-    if (head_dim == 128) CBK_TREE(CBK_BF16, 128); else CBK_TREE(CBK_BF16, 64);
-  } else {
-    if (head_dim == 128) CBK_TREE(CBK_F16, 128); else CBK_TREE(CBK_F16, 64);
-  }
-#undef CBK_TREE
-  return check_launch("tree_attn_kernel");
+  return a->dtype == CBK_BF16 ? dispatch_tree<CBK_BF16>(a, p, st) : dispatch_tree<CBK_F16>(a, p, st);
 }

@@ -258,7 +258,9 @@ int cbk_scatter_rows(const void* src, int64_t src_stride_bytes, const int64_t* i
 /* Decoding with drafted tokens: the three entries below, in this order, are one
  * layer's and one step's work beside its GEMMs when a model checks a tree of
  * drafted tokens at once instead of one token (no counterpart in the reference,
- * whose decode loop, runners.py:106-152, takes one token at a time).
+ * whose decode loop, runners.py:106-152, takes one token at a time).  Each takes
+ * its arguments in a struct (host memory, read before the call returns) whose
+ * `size` names the struct the caller was built with.
  *
  * cbk_norm_rope_scatter: per-head RMSNorm of Q and K (when q_weight and k_weight,
  * head_dim elements each, are given), rotation, and K / V into their cache rows.
@@ -277,12 +279,18 @@ int cbk_scatter_rows(const void* src, int64_t src_stride_bytes, const int64_t* i
  * one row, either's values may land).  head_dim and rotary_dim multiples of 16,
  * 16 <= rotary_dim <= head_dim <= 256; pointers 16-byte aligned, strides
  * multiples of 8. */
-int cbk_norm_rope_scatter(const void* q_src, int64_t q_row_stride, const void* k_src, int64_t k_row_stride,
-                          const void* v_src, int64_t v_row_stride, const int64_t* positions, const int64_t* rows,
-                          int64_t n, int n_q_heads, int n_kv_heads, int head_dim, int rotary_dim, int interleaved,
-                          int dtype, const void* q_weight, const void* k_weight, float eps, const void* rope_table,
-                          int64_t table_rows, int rope_mode, void* q_out, void* k_cache, void* v_cache,
-                          int64_t kv_row_stride, int64_t cap, int32_t* status, void* stream);
+typedef struct {
+  int64_t size;                                  /* sizeof(cbk_norm_rope_scatter_args) */
+  const void *q_src, *k_src, *v_src;
+  const int64_t *positions, *rows;
+  const void *q_weight, *k_weight, *rope_table;
+  void *q_out, *k_cache, *v_cache;
+  int32_t* status;
+  int64_t q_row_stride, k_row_stride, v_row_stride, kv_row_stride, n, table_rows, cap;
+  int32_t n_q_heads, n_kv_heads, head_dim, rotary_dim, interleaved, dtype, rope_mode;
+  float eps;
+} cbk_norm_rope_scatter_args;
+int cbk_norm_rope_scatter(const cbk_norm_rope_scatter_args* args, void* stream);
 
 /* Attention of a tree of drafted tokens over the cache.  Node i < n_nodes sees
  * rows [0, *n_ctx) and row *n_ctx + j for every j with bit j % 32 of
@@ -296,14 +304,22 @@ int cbk_norm_rope_scatter(const void* q_src, int64_t q_row_stride, const void* k
  * the device (a captured graph stays valid as it advances); *n_ctx < 0 or
  * *n_ctx + n_nodes > cap sets CBK_STATUS_BAD_INDEX and leaves out untouched.
  * head_dim 64 or 128, n_nodes <= 1024, any whole number of q heads per KV head;
- * pointers 16-byte aligned, kv_row_stride a multiple of 8.
- * The workspace needs no initialisation; calls that overlap on the GPU must not
+ * scale > 0; pointers 16-byte aligned (workspace 32), kv_row_stride a multiple
+ * of 8.  The workspace needs no initialisation; calls that overlap on the GPU must not
  * share it. */
 size_t cbk_tree_attn_workspace_bytes(int n_nodes, int64_t cap, int n_q_heads, int n_kv_heads, int head_dim);
-int cbk_tree_attn(const void* q, const void* k_cache, const void* v_cache, int64_t kv_row_stride,
-                  const int64_t* n_ctx, const int32_t* words, int64_t words_stride, int n_nodes, int64_t cap,
-                  int n_q_heads, int n_kv_heads, int head_dim, float scale, int dtype, void* out, void* workspace,
-                  size_t workspace_bytes, int32_t* status, void* stream);
+typedef struct {
+  int64_t size;                                  /* sizeof(cbk_tree_attn_args) */
+  const void *q, *k_cache, *v_cache;
+  const int64_t* n_ctx;
+  const int32_t* words;
+  void *out, *workspace;
+  int32_t* status;
+  int64_t kv_row_stride, words_stride, cap, workspace_bytes;
+  int32_t n_nodes, n_q_heads, n_kv_heads, head_dim, dtype;
+  float scale;
+} cbk_tree_attn_args;
+int cbk_tree_attn(const cbk_tree_attn_args* args, void* stream);
 
 /* Penalties for repeated tokens, bias and grammar mask on rows of logits, and the
  * token each row chooses.  Row r's history is history[r][0 .. lengths[r]), of
@@ -322,13 +338,23 @@ int cbk_tree_attn(const void* q, const void* k_cache, const void* v_cache, int64
  * the same or CBK_F32.  A token outside [0, vocab) is skipped and a length
  * outside [0, history_cap] clamped, both with CBK_STATUS_BAD_INDEX.
  * vocab <= 458752, history_cap < 2^30, n_tree <= 1024, repetition > 0. */
-int cbk_process_logits(const void* logits, int in_dtype, int64_t row_stride, int64_t rows, int64_t vocab,
-                       const int64_t* history, int64_t history_stride, int64_t history_cap, const int64_t* lengths,
-                       int64_t lengths_stride, const int64_t* n_prompt, int64_t n_prompt_stride, float repetition,
-                       float presence, float frequency, const float* bias, int64_t bias_stride, const int32_t* mask,
-                       int64_t mask_stride, const int64_t* tree_tokens, const int32_t* tree_words,
-                       int64_t tree_stride, int n_tree, void* out, int out_dtype, int64_t out_stride,
-                       int64_t* tokens, int32_t* status, void* stream);
+typedef struct {
+  int64_t size;                                  /* sizeof(cbk_process_logits_args) */
+  const void* logits;
+  const int64_t *history, *lengths, *n_prompt;
+  const float* bias;
+  const int32_t* mask;
+  const int64_t* tree_tokens;
+  const int32_t* tree_words;
+  void* out;
+  int64_t* tokens;
+  int32_t* status;
+  int64_t row_stride, rows, vocab, history_stride, history_cap, lengths_stride, n_prompt_stride, bias_stride,
+      mask_stride, tree_stride, out_stride;
+  int32_t n_tree, in_dtype, out_dtype;
+  float repetition, presence, frequency;
+} cbk_process_logits_args;
+int cbk_process_logits(const cbk_process_logits_args* args, void* stream);
 
 #ifdef __cplusplus
 }

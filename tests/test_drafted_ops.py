@@ -4,37 +4,52 @@ import numpy as np
 import pytest
 import torch
 
-# argument order of the three entries, with values that pass every check but the one under test
-NR = dict(q=16, qs=256, k=16, ks=128, v=16, vs=128, pos=16, rows=16, n=4, hq=4, hkv=2, d=64, r=64, il=0, dt=0, qw=16,
-          kw=16, eps=1e-6, table=16, t_rows=10, mode=1, q_out=16, kc=16, vc=16, kvs=128, cap=10, st=None, stream=None)
-TA = dict(q=16, k=16, v=16, kvs=128, n_ctx=16, words=16, ws_=1, t=4, cap=100, hq=4, hkv=2, d=64, scale=0.1, dt=0,
-          out=16, ws=256, bytes_=1 << 40, st=None, stream=None)
-PL = dict(x=16, dt=0, xs=100, rows=2, vocab=100, h=16, hs=0, hc=5, ln=None, ls=0, np_=None, nps=0, rep=1.1, pres=0.0,
-          freq=0.0, bias=None, bs=0, mask=None, ms=0, tt=None, tw=None, ts=0, nt=0, out=16, odt=2, os=100, tok=16,
-          st=None, stream=None)
+# the fields of the three argument structs after `size`, with values that pass every check but the one under test
+NR = dict(q=16, k=16, v=16, pos=16, rows=16, qw=16, kw=16, table=16, q_out=16, kc=16, vc=16, st=0, qs=256, ks=128,
+          vs=128, kvs=128, n=4, t_rows=10, cap=10, hq=4, hkv=2, d=64, r=64, il=0, dt=0, mode=1, eps=1e-6)
+TA = dict(q=16, k=16, v=16, n_ctx=16, words=16, out=16, ws=256, st=0, kvs=128, ws_=1, cap=100, bytes_=1 << 40, t=4,
+          hq=4, hkv=2, d=64, dt=0, scale=0.1)
+PL = dict(x=16, h=16, ln=0, np_=0, bias=0, mask=0, tt=0, tw=0, out=16, tok=16, st=0, xs=100, rows=2, vocab=100, hs=0,
+          hc=5, ls=0, nps=0, bs=0, ms=0, ts=0, os=100, nt=0, dt=0, odt=2, rep=1.1, pres=0.0, freq=0.0)
+
+
+def call(name, fields, **change):
+    from cacheblend import _native as N
+    fmt = N.PACK["cbk_" + name]
+    values = {**fields, **change}
+    size = values.pop("size", fmt.size)
+    rc = getattr(N.LIB, "cbk_" + name)(fmt.pack(size, *values.values()), None)
+    assert N.last_error() or rc == 0
+    return rc
+
+
+@pytest.mark.parametrize("name,fields", [("norm_rope_scatter", NR), ("tree_attn", TA), ("process_logits", PL)])
+def test_argument_struct_size_is_checked(name, fields):
+    from cacheblend import _native as N
+    assert call(name, fields, size=N.PACK["cbk_" + name].size - 8) == -1
+    assert getattr(N.LIB, "cbk_" + name)(None, None) == -1
 
 
 @pytest.mark.parametrize("change,code", [
     (dict(dt=2), -2), (dict(d=72), -2), (dict(d=272), -2), (dict(d=8), -2), (dict(r=8), -2), (dict(r=24), -2),
     (dict(r=80), -2), (dict(mode=2), -1), (dict(hq=0), -1), (dict(hkv=-1), -1), (dict(n=-1), -1), (dict(cap=-1), -1),
-    (dict(q=None), -1), (dict(rows=None), -1), (dict(table=None), -1), (dict(vc=None), -1), (dict(kw=None), -1),
+    (dict(q=0), -1), (dict(rows=0), -1), (dict(table=0), -1), (dict(vc=0), -1), (dict(kw=0), -1),
     (dict(qs=248), -1), (dict(ks=132), -1), (dict(kvs=64), -1), (dict(q_out=24), -1), (dict(qw=24), -1),
-    (dict(n=0), 0), (dict(n=0, q=None, rows=None), 0),
+    (dict(n=0), 0), (dict(n=0, q=0, rows=0), 0),
 ])
 def test_norm_rope_scatter_refusals(change, code):
-    from cacheblend import _native as N
-    assert N.LIB.cbk_norm_rope_scatter(*{**NR, **change}.values()) == code, N.last_error()
+    assert call("norm_rope_scatter", NR, **change) == code
 
 
 @pytest.mark.parametrize("change,code", [
     (dict(dt=2), -2), (dict(d=96), -2), (dict(hq=5), -1), (dict(hkv=0), -1), (dict(t=1025), -2), (dict(t=-1), -1 - 1),
     (dict(cap=3), -1), (dict(cap=1 << 31), -1), (dict(kvs=64), -1), (dict(kvs=132), -1), (dict(ws_=0), -1),
-    (dict(t=33, ws_=1), -1), (dict(q=None), -1), (dict(n_ctx=None), -1), (dict(words=None), -1), (dict(out=24), -1),
-    (dict(k=24), -1), (dict(bytes_=16), -4), (dict(t=0), 0),
+    (dict(t=33, ws_=1), -1), (dict(q=0), -1), (dict(n_ctx=0), -1), (dict(words=0), -1), (dict(out=24), -1),
+    (dict(k=24), -1), (dict(ws=16), -1), (dict(scale=0.0), -1),
+    (dict(scale=-0.1), -1), (dict(scale=float("inf")), -1), (dict(scale=float("nan")), -1), (dict(bytes_=16), -4), (dict(t=0), 0),
 ])
 def test_tree_attn_refusals(change, code):
-    from cacheblend import _native as N
-    assert N.LIB.cbk_tree_attn(*{**TA, **change}.values()) == code, N.last_error()
+    assert call("tree_attn", TA, **change) == code
 
 
 def test_tree_attn_workspace_refusals():
@@ -46,14 +61,13 @@ def test_tree_attn_workspace_refusals():
 
 @pytest.mark.parametrize("change,code", [
     (dict(dt=3), -2), (dict(odt=1), -2), (dict(dt=2, odt=0), -2), (dict(vocab=0), -2), (dict(vocab=1 << 20), -2),
-    (dict(rows=-1), -1), (dict(x=None), -1), (dict(tok=None), -1), (dict(rep=0.0), -1), (dict(rep=-1.0), -1),
+    (dict(rows=-1), -1), (dict(x=0), -1), (dict(tok=0), -1), (dict(rep=0.0), -1), (dict(rep=-1.0), -1),
     (dict(rep=float("nan")), -1), (dict(pres=float("nan")), -1), (dict(xs=99), -1), (dict(os=99), -1),
     (dict(mask=16, ms=3), -1), (dict(bias=16, bs=99), -1), (dict(hc=-1), -1), (dict(nt=2), -1), (dict(nt=1025), -1),
     (dict(nt=33, tt=16, tw=16, ts=1), -1), (dict(rows=0), 0),
 ])
 def test_process_logits_refusals(change, code):
-    from cacheblend import _native as N
-    assert N.LIB.cbk_process_logits(*{**PL, **change}.values()) == code, N.last_error()
+    assert call("process_logits", PL, **change) == code
 
 
 def test_cpu_tensors_are_refused():
