@@ -27,8 +27,9 @@ int check_launch(const char* what) {
 // cudaFuncSetAttribute applies to the current device; remember per (function, device).
 int ensure_smem_attr(const void* func, int bytes) {
   static std::mutex mu;
-  static const void* funcs[64];
-  static uint64_t done[64];
+  constexpr int kFuncs = 128;
+  static const void* funcs[kFuncs];
+  static uint64_t done[kFuncs];
   static int n_funcs = 0;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
@@ -38,7 +39,7 @@ int ensure_smem_attr(const void* func, int bytes) {
   for (int i = 0; i < n_funcs; ++i)
     if (funcs[i] == func) slot = i;
   if (slot < 0) {
-    if (n_funcs == 64) return set_error(CBK_ERR_CUDA, "attribute table full");
+    if (n_funcs == kFuncs) return set_error(CBK_ERR_CUDA, "attribute table full");
     slot = n_funcs++;
     funcs[slot] = func;
     done[slot] = 0;

@@ -12,12 +12,20 @@
 // is the first largest x, NaN counting as larger than any number; a row whose
 // mask allows nothing is all -inf and chooses token 0.
 //
-// A cluster of CTAs takes a row, each CTA a contiguous segment of the vocabulary,
+// A cluster of CTAs takes a row (several rows, one after the other, when there are
+// more rows than clusters fit), each CTA a contiguous segment of the vocabulary,
 // whose counts it keeps in its shared memory (bits 0-30 made, bit 31 in the
-// prompt).  The history is read once per row: the CTAs share its positions and
-// add to the owner's counts through distributed shared memory.  The row's choice
-// is a maximum over 64-bit keys (order of x, then lowest index) in the CTA and
-// over the cluster: one launch, no workspace, no order of atomics that could show.
+// prompt).  The history is read once per row -- once per cluster when the rows
+// share it -- the CTAs sharing its positions and adding to the owner's counts
+// through distributed shared memory; a tree node's path is added for its row and
+// taken back after it.  The row's choice is a maximum over 64-bit keys (order of x,
+// then lowest index) in the CTA and over the cluster: one launch, no workspace, no
+// order of atomics that could show.
+//
+// Bound by memory for many rows, by latency for few: a thread takes vectors of 8
+// logits (16 or 32 bytes), kLgBatch loads in flight, the first batch before the
+// counting starts.  Rows that do not lie on 16-byte boundaries are read element by
+// element, neighbouring lanes on neighbouring elements.
 #include <algorithm>
 
 #include "cbk_common.cuh"
@@ -28,6 +36,8 @@ int ensure_smem_attr(const void* func, int bytes);   // cbk_api.cu
 
 constexpr int kLgThreads = 512;
 constexpr int kLgCluster = 8;
+constexpr int kLgBatch = 4;
+constexpr int kLgMaxClusters = 36;                      // two CTAs on each of 148 SMs, whole clusters
 constexpr int kLgMaxVocab = kLgCluster * 56 * 1024;   // a segment's counts fit in shared memory
 constexpr uint32_t kLgPrompt = 0x80000000u;
 
@@ -41,7 +51,7 @@ struct LogitsParams {
   int32_t* status;
   int64_t row_stride, out_stride, hist_stride, hist_cap, len_stride, prompt_stride, bias_stride, mask_stride,
       tree_stride;
-  int rows, vocab, seg, n_tree, counted;
+  int rows, vocab, seg, n_tree, counted, shared;
   float repetition, presence, frequency;
 };
 
@@ -77,88 +87,252 @@ __device__ __forceinline__ void store1(void* p, int64_t i, float x) {
   else static_cast<uint16_t*>(p)[i] = Elem<DT>::from_f(x);
 }
 
-template <int IN, int OUT>
-__global__ void __launch_bounds__(kLgThreads)
-process_logits_kernel(const LogitsParams p) {
-  extern __shared__ uint32_t s_count[];             // [seg] when the row has a history
-  __shared__ unsigned long long s_best[kLgThreads / 32];
-  __shared__ unsigned long long s_row[kLgCluster];  // rank 0: one key per CTA of the cluster
-  const int row = blockIdx.x / kLgCluster, rank = static_cast<int>(cluster_rank());
-  const int tid = threadIdx.x;
-  const int v0 = rank * p.seg, v1 = min(v0 + p.seg, p.vocab);
+// max that propagates NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
 
-  if (p.counted) {
-    for (int i = tid; i < p.seg; i += kLgThreads) s_count[i] = 0;
-    cluster_sync_all();                              // every CTA's counts are zero before any is added to
-    const uint32_t base = smem_u32(s_count);
-    auto add = [&](int64_t t, bool made) {
-      if (t < 0 || t >= p.vocab) {
-        report(p.status, CBK_STATUS_BAD_INDEX);
-        return;
-      }
-      const int owner = static_cast<int>(t) / p.seg;
-      const uint32_t a = map_rank(base + 4u * (static_cast<int>(t) - owner * p.seg), owner);
-      if (made) asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(a), "r"(1u) : "memory");
-      else asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(a), "r"(kLgPrompt) : "memory");
-    };
-    if (p.history) {
-      int64_t len = p.lengths ? p.lengths[row * p.len_stride] : p.hist_cap;
-      if (len < 0 || len > p.hist_cap) {
-        if (tid == 0) report(p.status, CBK_STATUS_BAD_INDEX);
-        len = len < 0 ? 0 : p.hist_cap;
-      }
-      const int64_t prompt = p.n_prompt ? p.n_prompt[row * p.prompt_stride] : 0;
-      const int64_t* h = p.history + row * p.hist_stride;
-      for (int64_t i = rank * kLgThreads + tid; i < len; i += kLgCluster * kLgThreads) add(h[i], i >= prompt);
-    }
-    for (int j = rank * kLgThreads + tid; j < p.n_tree; j += kLgCluster * kLgThreads)
-      if ((p.tree_words[row * p.tree_stride + j / 32] >> (j % 32)) & 1u) add(p.tree_tokens[j], true);
-  }
-  // counts are whole; and every CTA of the cluster runs before one stores into rank 0
-  cluster_sync_all();
-
-  unsigned long long best = 0;
-  for (int i = v0 + tid; i < v1; i += kLgThreads) {
-    float x = load1<IN>(p.logits, row * p.row_stride + i);
-    if (p.counted) {
-      const uint32_t n = s_count[i - v0], c = n & ~kLgPrompt;
-      if (n) x = x > 0.f ? __fdiv_rn(x, p.repetition) : __fmul_rn(x, p.repetition);
-      if (c) x = __fsub_rn(__fsub_rn(x, __fmul_rn(p.frequency, static_cast<float>(c))), p.presence);
-    }
-    if (p.bias) x = __fadd_rn(x, p.bias[row * p.bias_stride + i]);
-    if (p.mask && !((p.mask[row * p.mask_stride + i / 32] >> (i % 32)) & 1u)) x = -INFINITY;
-    if (p.out) store1<OUT>(p.out, row * p.out_stride + i, x);
-    const unsigned long long k = (static_cast<unsigned long long>(order_key(x)) << 32) | (0xffffffffu - i);
-    best = k > best ? k : best;
-  }
+// VEC consecutive logits of a row as they lie in memory
+template <int DT, int VEC>
+struct Raw {
+  static constexpr int kWords = DT == CBK_F32 ? VEC : (VEC + 1) / 2;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    if constexpr (VEC == 8) {
+      const uint4* v = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + i * (DT == CBK_F32 ? 4 : 2));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long k = __shfl_xor_sync(0xffffffffu, best, o);
-    best = k > best ? k : best;
+      for (int k = 0; k < kWords / 4; ++k) {
+        const uint4 x = v[k];
+        w[4 * k] = x.x;
+        w[4 * k + 1] = x.y;
+        w[4 * k + 2] = x.z;
+        w[4 * k + 3] = x.w;
+      }
+    } else if constexpr (DT == CBK_F32) {
+      w[0] = static_cast<const uint32_t*>(p)[i];
+    } else {
+      w[0] = static_cast<const uint16_t*>(p)[i];
+    }
   }
-  if ((tid & 31) == 0) s_best[tid >> 5] = best;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kLgThreads / 32; ++w) best = s_best[w] > best ? s_best[w] : best;
-    const uint32_t a = map_rank(smem_u32(&s_row[rank]), 0);
-    asm volatile("st.relaxed.cluster.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(best) : "memory");
+  __device__ __forceinline__ float at(int e) const {
+    if constexpr (DT == CBK_F32) return __uint_as_float(w[e]);
+    else return Elem<DT>::to_f(static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1))));
   }
-  cluster_sync_all();
-  if (rank == 0 && tid == 0) {
-    best = s_row[0];
-    for (int c = 1; c < kLgCluster; ++c) best = s_row[c] > best ? s_row[c] : best;
-    p.tokens[row] = 0xffffffffu - static_cast<uint32_t>(best);
+};
+
+template <int IN, int OUT, int VEC>
+__global__ void __launch_bounds__(kLgThreads, 2)
+process_logits_kernel(const LogitsParams p) {
+  constexpr int kBatch = VEC == 1 ? 8 : IN == CBK_F32 ? kLgBatch / 2 : kLgBatch;
+  extern __shared__ __align__(16) uint32_t s_count[];    // [seg] when the rows have a history
+  __shared__ unsigned long long s_best[kLgThreads / 32];
+  __shared__ unsigned long long s_row[kLgCluster];       // rank 0: one key per CTA of the cluster
+  const int rank = static_cast<int>(cluster_rank()), tid = threadIdx.x;
+  const int n_clusters = gridDim.x / kLgCluster;
+  const int v0 = rank * p.seg, v1 = min(v0 + p.seg, p.vocab);
+  const uint32_t base = smem_u32(s_count);
+
+  auto owner_address = [&](int64_t t) {
+    const int owner = static_cast<int>(t) / p.seg;
+    return map_rank(base + 4u * (static_cast<int>(t) - owner * p.seg), owner);
+  };
+  auto add = [&](int64_t t, bool made, uint32_t by) {
+    if (t < 0 || t >= p.vocab) {
+      report(p.status, CBK_STATUS_BAD_INDEX);
+      return;
+    }
+    const uint32_t a = owner_address(t);
+    if (made) asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(a), "r"(by) : "memory");
+    else asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(a), "r"(kLgPrompt) : "memory");
+  };
+  auto add_path = [&](int row, uint32_t by) {
+    for (int j = rank * kLgThreads + tid; j < p.n_tree; j += kLgCluster * kLgThreads)
+      if ((p.tree_words[row * p.tree_stride + j / 32] >> (j % 32)) & 1u) add(p.tree_tokens[j], true, by);
+  };
+
+  for (int row = blockIdx.x / kLgCluster, turn = 0; row < p.rows; row += n_clusters, ++turn) {
+    const char* in_row = static_cast<const char*>(p.logits) + row * p.row_stride * (IN == CBK_F32 ? 4 : 2);
+    // element i of the segment's batch b, vector k: neighbouring lanes on neighbouring vectors
+    auto elem = [&](int b, int k) { return v0 + ((b * kBatch + k) * kLgThreads + tid) * VEC; };
+    Raw<IN, VEC> raw[kBatch];
+    auto load_batch = [&](int b) {
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = elem(b, k);
+        if (i + VEC <= v1) raw[k].load(in_row, i);
+      }
+    };
+    load_batch(0);
+
+    if (p.counted) {
+      if (turn == 0 || !p.shared) {
+        for (int i = tid; i < p.seg / 4; i += kLgThreads) reinterpret_cast<uint4*>(s_count)[i] = make_uint4(0, 0, 0, 0);
+        cluster_sync_all();                          // every CTA's counts are zero before any is added to
+        if (p.history) {
+          int64_t len = p.lengths ? p.lengths[row * p.len_stride] : p.hist_cap;
+          const int64_t prompt = p.n_prompt ? p.n_prompt[row * p.prompt_stride] : 0;
+          if (len < 0 || len > p.hist_cap) {
+            if (tid == 0) report(p.status, CBK_STATUS_BAD_INDEX);
+            len = len < 0 ? 0 : p.hist_cap;
+          }
+          const int64_t* h = p.history + row * p.hist_stride;
+          constexpr int kStep = kLgCluster * kLgThreads;
+          for (int64_t i = rank * kLgThreads + tid; i < len; i += 4 * kStep) {
+            int64_t t[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[k] = i + k * kStep < len ? h[i + k * kStep] : 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (i + k * kStep < len) add(t[k], i + k * kStep >= prompt, 1u);
+          }
+        }
+        add_path(row, 1u);
+      } else {
+        // the last row's reads of the counts lie behind its closing cluster barrier
+        add_path(row - n_clusters, 0xffffffffu);
+        add_path(row, 1u);
+      }
+    }
+    // counts are whole; and every CTA of the cluster runs before one stores into rank 0
+    cluster_sync_all();
+
+    float best = -INFINITY;
+    int best_i = v0 + tid * VEC;                     // the thread's first element: the first of a row of -inf
+    auto finish = [&](float x, int i) {              // everything but the penalties, then the store
+      if (p.mask && !((p.mask[row * p.mask_stride + i / 32] >> (i % 32)) & 1u)) x = -INFINITY;
+      return x;
+    };
+    auto penalise = [&](float x, uint32_t n) {
+      if (n) {
+        x = x > 0.f ? __fdiv_rn(x, p.repetition) : __fmul_rn(x, p.repetition);
+        const uint32_t c = n & ~kLgPrompt;
+        if (c) x = __fsub_rn(__fsub_rn(x, __fmul_rn(p.frequency, static_cast<float>(c))), p.presence);
+      }
+      return x;
+    };
+    auto take = [&](float x, int i) {
+      if (x > best || (x != x && best == best)) {
+        best = x;
+        best_i = i;
+      }
+    };
+    const int n_batches = (p.seg + kBatch * kLgThreads * VEC - 1) / (kBatch * kLgThreads * VEC);
+    for (int b = 0; b < n_batches; ++b) {
+      if (b > 0) load_batch(b);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = elem(b, k);
+        if (i >= v1) continue;
+        if (VEC == 8 && i + VEC <= v1) {
+          float x[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) x[e] = raw[k].at(e);
+          if (p.counted) {
+            uint32_t n[VEC], any = 0;
+#pragma unroll
+            for (int q = 0; q < VEC / 4; ++q) {
+              const uint4 c4 = *reinterpret_cast<const uint4*>(s_count + (i - v0) + 4 * q);
+              n[4 * q] = c4.x;
+              n[4 * q + 1] = c4.y;
+              n[4 * q + 2] = c4.z;
+              n[4 * q + 3] = c4.w;
+              any |= c4.x | c4.y | c4.z | c4.w;
+            }
+            if (any) {
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) x[e] = penalise(x[e], n[e]);
+            }
+          }
+          if (p.bias) {
+            const float4* bv = reinterpret_cast<const float4*>(p.bias + row * p.bias_stride + i);
+#pragma unroll
+            for (int q = 0; q < VEC / 4; ++q) {
+              const float4 c4 = __ldg(bv + q);
+              x[4 * q] = __fadd_rn(x[4 * q], c4.x);
+              x[4 * q + 1] = __fadd_rn(x[4 * q + 1], c4.y);
+              x[4 * q + 2] = __fadd_rn(x[4 * q + 2], c4.z);
+              x[4 * q + 3] = __fadd_rn(x[4 * q + 3], c4.w);
+            }
+          }
+          if (p.mask) {
+            // i is a multiple of 8: the 8 bits are one byte of the row
+            const uint32_t bits = __ldg(reinterpret_cast<const uint8_t*>(p.mask + row * p.mask_stride) + i / 8);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) x[e] = (bits >> e) & 1u ? x[e] : -INFINITY;
+          }
+          float m = x[0];
+#pragma unroll
+          for (int e = 1; e < VEC; ++e) m = max_nan(m, x[e]);
+          if (!(m <= best)) {                        // larger, or NaN: rare after the first few
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) take(x[e], i + e);
+          }
+          if (p.out) {
+            if constexpr (OUT == CBK_F32) {
+              float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.out_stride + i);
+              o[0] = make_float4(x[0], x[1], x[2], x[3]);
+              o[1] = make_float4(x[4], x[5], x[6], x[7]);
+            } else {
+              st_vec(static_cast<uint16_t*>(p.out) + row * p.out_stride + i,
+                     make_uint4(Pk<OUT>::cvt(x[0], x[1]), Pk<OUT>::cvt(x[2], x[3]), Pk<OUT>::cvt(x[4], x[5]),
+                                Pk<OUT>::cvt(x[6], x[7])));
+            }
+          }
+        } else {
+          // a row's last, partial vector, or a row off the boundaries
+          for (int j = i; j < min(i + VEC, v1); ++j) {
+            float x = VEC == 1 ? raw[k].at(0) : load1<IN>(in_row, j);
+            if (p.counted) x = penalise(x, s_count[j - v0]);
+            if (p.bias) x = __fadd_rn(x, p.bias[row * p.bias_stride + j]);
+            x = finish(x, j);
+            take(x, j);
+            if (p.out) store1<OUT>(p.out, row * p.out_stride + j, x);
+          }
+        }
+      }
+    }
+    // a thread without an element has index >= vocab or another's: it must not win
+    unsigned long long key = best_i < v1
+        ? (static_cast<unsigned long long>(order_key(best)) << 32) | (0xffffffffu - static_cast<uint32_t>(best_i)) : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
+      key = other > key ? other : key;
+    }
+    if ((tid & 31) == 0) s_best[tid >> 5] = key;
+    __syncthreads();
+    if (tid < 32) {
+      key = tid < kLgThreads / 32 ? s_best[tid] : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
+        key = other > key ? other : key;
+      }
+      if (tid == 0) {
+        const uint32_t a = map_rank(smem_u32(&s_row[rank]), 0);
+        asm volatile("st.relaxed.cluster.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(key) : "memory");
+      }
+    }
+    cluster_sync_all();
+    if (rank == 0 && tid == 0) {
+      key = s_row[0];
+      for (int c = 1; c < kLgCluster; ++c) key = s_row[c] > key ? s_row[c] : key;
+      p.tokens[row] = 0xffffffffu - static_cast<uint32_t>(key);
+    }
   }
 }
 
-template <int IN, int OUT>
+template <int IN, int OUT, int VEC>
 static int launch_logits(const LogitsParams& p, cudaStream_t st) {
-  auto kern = process_logits_kernel<IN, OUT>;
+  auto kern = process_logits_kernel<IN, OUT, VEC>;
   const int smem = p.counted ? p.seg * 4 : 0;
   if (smem > 48 * 1024)
     if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), 224 * 1024)) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.rows) * kLgCluster);
+  const int turns = (p.rows + kLgMaxClusters - 1) / kLgMaxClusters;      // rows per cluster
+  cfg.gridDim = dim3(static_cast<unsigned>((p.rows + turns - 1) / turns) * kLgCluster);
   cfg.blockDim = dim3(kLgThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -228,14 +402,27 @@ extern "C" int cbk_process_logits(const cbk_process_logits_args* a, void* stream
   p.seg = static_cast<int>((a->vocab + kLgCluster * 32 - 1) / (kLgCluster * 32) * 32);
   p.n_tree = a->n_tree;
   p.counted = p.history != nullptr || a->n_tree > 0;
+  p.shared = p.history == nullptr || (a->history_stride == 0 && a->lengths_stride == 0 && a->n_prompt_stride == 0);
   p.repetition = a->repetition;
   p.presence = a->presence;
   p.frequency = a->frequency;
   auto st = static_cast<cudaStream_t>(stream);
   const bool f32 = a->out && a->out_dtype == CBK_F32;
+  // whole 16-byte vectors: every row of logits, output and bias starts on a boundary
+  const int in_size = a->in_dtype == CBK_F32 ? 4 : 2, out_size = f32 ? 4 : in_size;
+  const uint64_t off = reinterpret_cast<uintptr_t>(a->logits) | (a->rows > 1 ? a->row_stride * in_size : 0) |
+                       (a->out ? reinterpret_cast<uintptr_t>(a->out) | (a->rows > 1 ? a->out_stride * out_size : 0) : 0) |
+                       (a->bias ? reinterpret_cast<uintptr_t>(a->bias) | (a->bias_stride * 4) : 0);
+  const bool vec = (off & 15u) == 0;
+#define CBK_LG(IN, OUT) return vec ? launch_logits<IN, OUT, 8>(p, st) : launch_logits<IN, OUT, 1>(p, st)
   switch (a->in_dtype) {
-    case CBK_F32: return launch_logits<CBK_F32, CBK_F32>(p, st);
-    case CBK_BF16: return f32 ? launch_logits<CBK_BF16, CBK_F32>(p, st) : launch_logits<CBK_BF16, CBK_BF16>(p, st);
-    default: return f32 ? launch_logits<CBK_F16, CBK_F32>(p, st) : launch_logits<CBK_F16, CBK_F16>(p, st);
+    case CBK_F32: CBK_LG(CBK_F32, CBK_F32);
+    case CBK_BF16:
+      if (f32) CBK_LG(CBK_BF16, CBK_F32);
+      CBK_LG(CBK_BF16, CBK_BF16);
+    default:
+      if (f32) CBK_LG(CBK_F16, CBK_F32);
+      CBK_LG(CBK_F16, CBK_F16);
   }
+#undef CBK_LG
 }
