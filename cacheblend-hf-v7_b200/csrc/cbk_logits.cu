@@ -26,6 +26,9 @@
 // logits (16 or 32 bytes), kLgBatch loads in flight, the first batch before the
 // counting starts.  Rows that do not lie on 16-byte boundaries are read element by
 // element, neighbouring lanes on neighbouring elements.
+#ifndef LG_REMOTE
+#define LG_REMOTE 0
+#endif
 #include <algorithm>
 
 #include "cbk_common.cuh"
@@ -37,6 +40,7 @@ int ensure_smem_attr(const void* func, int bytes);   // cbk_api.cu
 constexpr int kLgThreads = 512;
 constexpr int kLgCluster = 8;
 constexpr int kLgBatch = 4;
+constexpr int kLgBlock = 128;                           // tokens of a CTA's blocks
 constexpr int kLgMaxClusters = 36;                      // two CTAs on each of 148 SMs, whole clusters
 constexpr int kLgMaxVocab = kLgCluster * 56 * 1024;   // a segment's counts fit in shared memory
 constexpr uint32_t kLgPrompt = 0x80000000u;
@@ -131,37 +135,51 @@ process_logits_kernel(const LogitsParams p) {
   __shared__ unsigned long long s_row[kLgCluster];       // rank 0: one key per CTA of the cluster
   const int rank = static_cast<int>(cluster_rank()), tid = threadIdx.x;
   const int n_clusters = gridDim.x / kLgCluster;
-  const int v0 = rank * p.seg, v1 = min(v0 + p.seg, p.vocab);
+#if LG_REMOTE
   const uint32_t base = smem_u32(s_count);
-
-  auto owner_address = [&](int64_t t) {
-    const int owner = static_cast<int>(t) / p.seg;
-    return map_rank(base + 4u * (static_cast<int>(t) - owner * p.seg), owner);
-  };
+#endif
+  // the CTA's share of the vocabulary: every kLgCluster-th block of kLgBlock tokens,
+  // one after the other at offsets [0, seg) of its counts
+  auto token_at = [&](int o) { return ((o / kLgBlock) * kLgCluster + rank) * kLgBlock + o % kLgBlock; };
   auto add = [&](int64_t t, bool made, uint32_t by) {
     if (t < 0 || t >= p.vocab) {
-      report(p.status, CBK_STATUS_BAD_INDEX);
+      if (rank == 0) report(p.status, CBK_STATUS_BAD_INDEX);
       return;
     }
-    const uint32_t a = owner_address(t);
+    const uint32_t block = static_cast<uint32_t>(t) / kLgBlock;
+    const uint32_t o = (block / kLgCluster) * kLgBlock + static_cast<uint32_t>(t) % kLgBlock;
+#if LG_REMOTE
+    const uint32_t a = map_rank(base + 4u * o, block % kLgCluster);
     if (made) asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(a), "r"(by) : "memory");
     else asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(a), "r"(kLgPrompt) : "memory");
+#else
+    if (block % kLgCluster != rank) return;
+    if (made) atomicAdd(s_count + o, by);
+    else atomicOr(s_count + o, kLgPrompt);
+#endif
   };
+#if LG_REMOTE
+  constexpr int kStep = kLgCluster * kLgThreads;
+  const int first = rank * kLgThreads + tid;
+#else
+  constexpr int kStep = kLgThreads;
+  const int first = tid;
+#endif
   auto add_path = [&](int row, uint32_t by) {
-    for (int j = rank * kLgThreads + tid; j < p.n_tree; j += kLgCluster * kLgThreads)
+    for (int j = first; j < p.n_tree; j += kStep)
       if ((p.tree_words[row * p.tree_stride + j / 32] >> (j % 32)) & 1u) add(p.tree_tokens[j], true, by);
   };
 
   for (int row = blockIdx.x / kLgCluster, turn = 0; row < p.rows; row += n_clusters, ++turn) {
     const char* in_row = static_cast<const char*>(p.logits) + row * p.row_stride * (IN == CBK_F32 ? 4 : 2);
-    // element i of the segment's batch b, vector k: neighbouring lanes on neighbouring vectors
-    auto elem = [&](int b, int k) { return v0 + ((b * kBatch + k) * kLgThreads + tid) * VEC; };
+    // offset of the thread's vector k of batch b: neighbouring lanes on neighbouring vectors
+    auto offset = [&](int b, int k) { return ((b * kBatch + k) * kLgThreads + tid) * VEC; };
     Raw<IN, VEC> raw[kBatch];
     auto load_batch = [&](int b) {
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
-        const int i = elem(b, k);
-        if (i + VEC <= v1) raw[k].load(in_row, i);
+        const int o = offset(b, k), i = token_at(o);
+        if (o < p.seg && i + VEC <= p.vocab) raw[k].load(in_row, i);
       }
     };
     load_batch(0);
@@ -178,13 +196,13 @@ process_logits_kernel(const LogitsParams p) {
             len = len < 0 ? 0 : p.hist_cap;
           }
           const int64_t* h = p.history + row * p.hist_stride;
-          constexpr int kStep = kLgCluster * kLgThreads;
-          for (int64_t i = rank * kLgThreads + tid; i < len; i += 4 * kStep) {
-            int64_t t[4];
+          constexpr int kAhead = 8;
+          for (int64_t i = first; i < len; i += kAhead * kStep) {
+            int64_t t[kAhead];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) t[k] = i + k * kStep < len ? h[i + k * kStep] : 0;
+            for (int k = 0; k < kAhead; ++k) t[k] = i + k * kStep < len ? __ldg(h + i + k * kStep) : 0;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < kAhead; ++k)
               if (i + k * kStep < len) add(t[k], i + k * kStep >= prompt, 1u);
           }
         }
@@ -199,7 +217,7 @@ process_logits_kernel(const LogitsParams p) {
     cluster_sync_all();
 
     float best = -INFINITY;
-    int best_i = v0 + tid * VEC;                     // the thread's first element: the first of a row of -inf
+    int best_i = token_at(tid * VEC);                     // the thread's first element: the first of a row of -inf
     auto finish = [&](float x, int i) {              // everything but the penalties, then the store
       if (p.mask && !((p.mask[row * p.mask_stride + i / 32] >> (i % 32)) & 1u)) x = -INFINITY;
       return x;
@@ -223,9 +241,9 @@ process_logits_kernel(const LogitsParams p) {
       if (b > 0) load_batch(b);
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
-        const int i = elem(b, k);
-        if (i >= v1) continue;
-        if (VEC == 8 && i + VEC <= v1) {
+        const int o = offset(b, k), i = token_at(o);
+        if (o >= p.seg || i >= p.vocab) continue;
+        if (VEC == 8 && i + VEC <= p.vocab) {
           float x[VEC];
 #pragma unroll
           for (int e = 0; e < VEC; ++e) x[e] = raw[k].at(e);
@@ -233,7 +251,7 @@ process_logits_kernel(const LogitsParams p) {
             uint32_t n[VEC], any = 0;
 #pragma unroll
             for (int q = 0; q < VEC / 4; ++q) {
-              const uint4 c4 = *reinterpret_cast<const uint4*>(s_count + (i - v0) + 4 * q);
+              const uint4 c4 = *reinterpret_cast<const uint4*>(s_count + o + 4 * q);
               n[4 * q] = c4.x;
               n[4 * q + 1] = c4.y;
               n[4 * q + 2] = c4.z;
@@ -271,9 +289,9 @@ process_logits_kernel(const LogitsParams p) {
           }
           if (p.out) {
             if constexpr (OUT == CBK_F32) {
-              float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.out_stride + i);
-              o[0] = make_float4(x[0], x[1], x[2], x[3]);
-              o[1] = make_float4(x[4], x[5], x[6], x[7]);
+              float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.out_stride + i);
+              dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+              dst[1] = make_float4(x[4], x[5], x[6], x[7]);
             } else {
               st_vec(static_cast<uint16_t*>(p.out) + row * p.out_stride + i,
                      make_uint4(Pk<OUT>::cvt(x[0], x[1]), Pk<OUT>::cvt(x[2], x[3]), Pk<OUT>::cvt(x[4], x[5]),
@@ -282,9 +300,9 @@ process_logits_kernel(const LogitsParams p) {
           }
         } else {
           // a row's last, partial vector, or a row off the boundaries
-          for (int j = i; j < min(i + VEC, v1); ++j) {
+          for (int j = i; j < min(i + VEC, p.vocab); ++j) {
             float x = VEC == 1 ? raw[k].at(0) : load1<IN>(in_row, j);
-            if (p.counted) x = penalise(x, s_count[j - v0]);
+            if (p.counted) x = penalise(x, s_count[o + j - i]);
             if (p.bias) x = __fadd_rn(x, p.bias[row * p.bias_stride + j]);
             x = finish(x, j);
             take(x, j);
@@ -294,7 +312,7 @@ process_logits_kernel(const LogitsParams p) {
       }
     }
     // a thread without an element has index >= vocab or another's: it must not win
-    unsigned long long key = best_i < v1
+    unsigned long long key = tid * VEC < p.seg && best_i < p.vocab
         ? (static_cast<unsigned long long>(order_key(best)) << 32) | (0xffffffffu - static_cast<uint32_t>(best_i)) : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -399,7 +417,7 @@ extern "C" int cbk_process_logits(const cbk_process_logits_args* a, void* stream
   p.tree_stride = a->tree_stride;
   p.rows = static_cast<int>(a->rows);
   p.vocab = static_cast<int>(a->vocab);
-  p.seg = static_cast<int>((a->vocab + kLgCluster * 32 - 1) / (kLgCluster * 32) * 32);
+  p.seg = static_cast<int>((a->vocab + kLgCluster * kLgBlock - 1) / (kLgCluster * kLgBlock) * kLgBlock);
   p.n_tree = a->n_tree;
   p.counted = p.history != nullptr || a->n_tree > 0;
   p.shared = p.history == nullptr || (a->history_stride == 0 && a->lengths_stride == 0 && a->n_prompt_stride == 0);
