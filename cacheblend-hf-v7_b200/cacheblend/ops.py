@@ -494,21 +494,32 @@ def scatter_rows(src: torch.Tensor, idx: torch.Tensor, n_rows: int, out: torch.T
 _DT3 = {**_DT, torch.float32: N.CBK_F32}
 
 
-def _call(name: str, dev: torch.device, n_launches: int, *args) -> None:
-    """One C-ABI call with its packed argument struct on dev's current stream, with
-    dev the current device meanwhile and its span timed when timing is on."""
-    name_c = "cbk_" + name
-    fmt = N.PACK[name_c]
-    packed = fmt.pack(fmt.size, *args)
-    fn = getattr(N.LIB, name_c)
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if TIMES.active or torch.cuda.current_device() != dev.index:
-        with torch.cuda.device(dev), TIMES.span(name, dev, n_launches):
-            rc = fn(packed, stream)
-    else:
-        rc = fn(packed, stream)
-    if rc:
-        N.check(rc, name_c)
+def _launcher(name: str, n_launches: int):
+    """Caller of one C-ABI entry that takes a packed argument struct: on dev's
+    current stream, with dev the current device meanwhile and the span timed when
+    timing is on.  (What it needs is looked up once: these calls are short enough
+    for the lookups to show.)"""
+    entry = "cbk_" + name
+    fmt = N.PACK[entry]
+    pack, size, fn = fmt.pack, fmt.size, getattr(N.LIB, entry)
+    raw_stream, current_device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+
+    def launch(dev: torch.device, *args) -> None:
+        index = dev.index
+        packed = pack(size, *args)
+        if TIMES.active or current_device() != index:
+            with torch.cuda.device(dev), TIMES.span(name, dev, n_launches):
+                rc = fn(packed, raw_stream(index))
+        else:
+            rc = fn(packed, raw_stream(index))
+        if rc:
+            N.check(rc, entry)
+    return launch
+
+
+_norm_rope_scatter = _launcher("norm_rope_scatter", 1)
+_tree_attn = _launcher("tree_attn", 2)
+_process_logits = _launcher("process_logits", 1)
 
 
 def _same_device(first: torch.Tensor, *others) -> torch.device:
@@ -522,21 +533,19 @@ def _same_device(first: torch.Tensor, *others) -> torch.device:
     return first.device
 
 
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _src_rows(t: torch.Tensor, n: int, cols: int, who: str) -> torch.Tensor:
-    """t as n rows of cols elements, in place where its rows can be read as they are."""
+def _src_rows(t: torch.Tensor, n: int, cols: int, who: str) -> tuple[torch.Tensor, int]:
+    """(t as n rows of cols elements, row stride), in place where its rows can be read as they are."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.shape[0] != n or t.shape[1] != cols:
+    if t.shape != (n, cols):
         raise ValueError(f"{who} must be {n} rows of {cols}, got {list(t.shape)}")
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < cols or t.data_ptr() % 16:
+    row, col = t.stride()
+    if col != 1 or row % 8 or row < cols or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-    return t
+        row = cols
+    return t, row
 
 
 def _index(t: torch.Tensor, n: int, who: str) -> torch.Tensor:
@@ -545,13 +554,15 @@ def _index(t: torch.Tensor, n: int, who: str) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, kv_dim: int, who: str) -> None:
+def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, kv_dim: int, who: str) -> tuple[int, int]:
+    """(rows, row stride) of the caches."""
     if k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise ValueError(f"{who}: caches must be {dtype}, got {k_cache.dtype} / {v_cache.dtype}")
-    if (k_cache.dim() != 2 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride()
-            or k_cache.shape[1] != kv_dim or k_cache.stride(1) != 1):
+    shape, stride = k_cache.shape, k_cache.stride()
+    if len(shape) != 2 or shape != v_cache.shape or stride != v_cache.stride() or shape[1] != kv_dim or stride[1] != 1:
         raise ValueError(f"{who}: k_cache and v_cache must be rows of {kv_dim} elements with one layout, got "
-                         f"{list(k_cache.shape)} and {list(v_cache.shape)}")
+                         f"{list(shape)} and {list(v_cache.shape)}")
+    return shape[0], stride[0]
 
 
 def norm_rope_scatter(q_src: torch.Tensor, k_src: torch.Tensor, v_src: torch.Tensor, positions: torch.Tensor,
@@ -575,36 +586,40 @@ def norm_rope_scatter(q_src: torch.Tensor, k_src: torch.Tensor, v_src: torch.Ten
     dev = _same_device(q_src, k_src, v_src, positions, rows, rope, k_cache, v_cache, q_weight, k_weight, q_out,
                        status)
     dt = q_src.dtype
-    code = dtype_code(dt)
+    code = _DT.get(dt)
+    if code is None:
+        dtype_code(dt)
     if mode not in ROPE_MODES:
         raise ValueError(f"norm_rope_scatter: mode must be one of {sorted(ROPE_MODES)}, got {mode!r}")
     if k_src.dtype != dt or v_src.dtype != dt:
         raise ValueError(f"norm_rope_scatter: q, k and v must have one dtype, got {dt}, {k_src.dtype}, {v_src.dtype}")
     n, qd, kd = rows.numel(), n_q_heads * head_dim, n_kv_heads * head_dim
-    q2 = _src_rows(q_src, n, qd, "norm_rope_scatter: q_src")
-    k2 = _src_rows(k_src, n, kd, "norm_rope_scatter: k_src")
-    v2 = _src_rows(v_src, n, kd, "norm_rope_scatter: v_src")
+    q2, qs = _src_rows(q_src, n, qd, "norm_rope_scatter: q_src")
+    k2, ks = _src_rows(k_src, n, kd, "norm_rope_scatter: k_src")
+    v2, vs = _src_rows(v_src, n, kd, "norm_rope_scatter: v_src")
     positions = _index(positions, n, "norm_rope_scatter: positions")
     rows = _index(rows, n, "norm_rope_scatter: rows")
-    if rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or not rope.is_contiguous():
+    table = rope.shape
+    if rope.dtype != torch.float32 or len(table) != 3 or table[2] != 2 or not rope.is_contiguous():
         raise ValueError("norm_rope_scatter: rope must be a contiguous fp32 table [n_pos][R / 2][2]")
-    _check_cache(k_cache, v_cache, dt, kd, "norm_rope_scatter")
-    if (q_weight is None) != (k_weight is None):
-        raise ValueError("norm_rope_scatter: give both q_weight and k_weight, or neither")
-    if q_weight is not None:
+    cap, kvs = _check_cache(k_cache, v_cache, dt, kd, "norm_rope_scatter")
+    qw = kw = 0
+    if q_weight is not None and k_weight is not None:
         for w in (q_weight, k_weight):
             if w.dtype != dt or w.numel() != head_dim or not w.is_contiguous():
                 raise ValueError(f"norm_rope_scatter: weights must be contiguous {dt}[{head_dim}], got "
                                  f"{w.dtype}{list(w.shape)}")
+        qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
+    elif q_weight is not None or k_weight is not None:
+        raise ValueError("norm_rope_scatter: give both q_weight and k_weight, or neither")
     if q_out is None:
-        q_out = torch.empty((n, qd), dtype=dt, device=dev)
+        q_out = q2.new_empty((n, qd))
     elif q_out.dtype != dt or q_out.numel() != n * qd or not q_out.is_contiguous():
         raise ValueError(f"norm_rope_scatter: q_out must be contiguous {dt} with {n} rows of {qd}")
-    _call("norm_rope_scatter", dev, 1, q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), positions.data_ptr(),
-          rows.data_ptr(), _ptr(q_weight), _ptr(k_weight), rope.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
-          v_cache.data_ptr(), _ptr(status), q2.stride(0), k2.stride(0), v2.stride(0), k_cache.stride(0), n,
-          rope.shape[0], k_cache.shape[0], n_q_heads, n_kv_heads, head_dim, 2 * rope.shape[1], bool(interleaved), code,
-          ROPE_MODES[mode], eps)
+    _norm_rope_scatter(dev, q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), positions.data_ptr(), rows.data_ptr(), qw, kw,
+                       rope.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                       0 if status is None else status.data_ptr(), qs, ks, vs, kvs, n, table[0], cap, n_q_heads,
+                       n_kv_heads, head_dim, 2 * table[1], bool(interleaved), code, ROPE_MODES[mode], eps)
     return q_out
 
 
@@ -614,8 +629,11 @@ def tree_workspace(n_nodes: int, cap: int, n_q_heads: int, n_kv_heads: int, head
     if head_dim not in (64, 128) or n_nodes > 1024:
         raise NotImplementedError(f"tree_attn: head_dim 64 or 128 and at most 1024 nodes, got {head_dim}, {n_nodes}")
     device = torch.device(device)
-    with torch.cuda.device(device):
+    if device.index is None or torch.cuda.current_device() == device.index:
         nbytes = N.LIB.cbk_tree_attn_workspace_bytes(n_nodes, cap, n_q_heads, n_kv_heads, head_dim)
+    else:
+        with torch.cuda.device(device):          # sized for that device's SMs
+            nbytes = N.LIB.cbk_tree_attn_workspace_bytes(n_nodes, cap, n_q_heads, n_kv_heads, head_dim)
     if nbytes == 0:
         raise ValueError(f"tree_workspace: {N.last_error()}")
     return torch.empty((nbytes,), dtype=torch.uint8, device=device)
@@ -634,31 +652,32 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_c
     leaves ``out`` as it was."""
     dev = _same_device(q, k_cache, v_cache, n_ctx, words, workspace, out, status)
     dt = q.dtype
-    code = dtype_code(dt)
-    t, qd = words.shape[0], n_q_heads * head_dim
-    if words.dtype != torch.int32 or words.dim() != 2 or words.shape[1] * 32 < t or words.stride(1) != 1:
-        raise ValueError(f"tree_attn: words must be int32 [T][>= ceil(T / 32)] rows, got "
-                         f"{words.dtype}{list(words.shape)}")
+    code = _DT.get(dt)
+    if code is None:
+        dtype_code(dt)
+    ws, qd = words.shape, n_q_heads * head_dim
+    if words.dtype != torch.int32 or len(ws) != 2 or ws[1] * 32 < ws[0] or words.stride(1) != 1:
+        raise ValueError(f"tree_attn: words must be int32 [T][>= ceil(T / 32)] rows, got {words.dtype}{list(ws)}")
+    t = ws[0]
     if q.numel() != t * qd or q.shape[-1] != qd:
         raise ValueError(f"tree_attn: q must be {t} rows of {qd}, got {list(q.shape)}")
     if n_ctx.dtype != torch.int64 or n_ctx.numel() != 1:
         raise ValueError("tree_attn: n_ctx must be one int64 on the device")
-    _check_cache(k_cache, v_cache, dt, n_kv_heads * head_dim, "tree_attn")
+    cap, kvs = _check_cache(k_cache, v_cache, dt, n_kv_heads * head_dim, "tree_attn")
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     words, words_stride = _word_rows(words)
-    cap = k_cache.shape[0]
     if workspace is None:
         workspace = tree_workspace(t, cap, n_q_heads, n_kv_heads, head_dim, dev)
     elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise ValueError("tree_attn: workspace must come from tree_workspace")
     if out is None:
-        out = torch.empty((t, qd), dtype=dt, device=dev)
+        out = torch.empty_like(q).view(t, qd) if q.dim() != 2 else torch.empty_like(q)
     elif out.dtype != dt or out.numel() != t * qd or not out.is_contiguous():
         raise ValueError(f"tree_attn: out must be contiguous {dt} with {t} rows of {qd}")
-    _call("tree_attn", dev, 2, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), n_ctx.data_ptr(),
-          words.data_ptr(), out.data_ptr(), workspace.data_ptr(), _ptr(status), k_cache.stride(0), words_stride, cap,
-          workspace.numel(), t, n_q_heads, n_kv_heads, head_dim, code, scale)
+    _tree_attn(dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), n_ctx.data_ptr(), words.data_ptr(),
+               out.data_ptr(), workspace.data_ptr(), 0 if status is None else status.data_ptr(), kvs, words_stride,
+               cap, workspace.numel(), t, n_q_heads, n_kv_heads, head_dim, code, scale)
     return out
 
 
@@ -694,15 +713,18 @@ def _word_rows(words: torch.Tensor) -> tuple[torch.Tensor, int]:
     return words, words.stride(0)
 
 
-def _row_stride(t: torch.Tensor, rows: int, cols: int, who: str) -> tuple[torch.Tensor, int]:
-    """t as [rows][>= cols] or one shared row; (tensor with unit inner stride, row stride or 0)."""
-    if t.dim() == 1:
-        t = t.unsqueeze(0)
-    if t.dim() != 2 or t.shape[0] not in (1, rows) or t.shape[1] < cols:
+def _row_stride(t: torch.Tensor, rows: int, cols: int, who: str) -> tuple[torch.Tensor, int, int]:
+    """t as [rows][>= cols] or one shared row: (tensor with unit inner stride, row length, row stride or 0)."""
+    shape = t.shape
+    if len(shape) == 1:
+        shape = (1, shape[0])
+    if len(shape) != 2 or (shape[0] != 1 and shape[0] != rows) or shape[1] < cols:
         raise ValueError(f"{who} must be one row or {rows} rows of at least {cols}, got {list(t.shape)}")
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    stride = t.stride()
+    if stride[-1] != 1 and shape[1] > 1:
         t = t.contiguous()
-    return t, (0 if t.shape[0] == 1 else t.stride(0))
+        stride = t.stride()
+    return t, shape[1], (0 if shape[0] == 1 else stride[0])
 
 
 def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
@@ -727,67 +749,82 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, le
     chooses 0.  ``out`` may be ``logits``; ``out_dtype`` is the logits' (default)
     or fp32."""
     dev = _same_device(logits, history, lengths, n_prompt, bias, mask_words, tree_tokens, tree_words, out, status)
-    if logits.dtype not in _DT3:
-        raise NotImplementedError(f"process_logits: bf16, fp16 or fp32 logits, got {logits.dtype}")
+    dt = logits.dtype
+    code = _DT3.get(dt)
+    if code is None:
+        raise NotImplementedError(f"process_logits: bf16, fp16 or fp32 logits, got {dt}")
     shape = logits.shape
-    if logits.dim() != 2:
+    flat = len(shape) == 2
+    if not flat:
         logits = logits.reshape(-1, shape[-1])
     rows, vocab = logits.shape
-    if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
+    row_stride, col = logits.stride()
+    if col != 1 or (rows > 1 and row_stride < vocab):
         logits = logits.contiguous()
+        row_stride = vocab
+    hist = lens = prompt = bias_p = mask_p = toks = words = 0
     hist_stride = hist_cap = len_stride = prompt_stride = bias_stride = mask_stride = tree_stride = n_tree = 0
-    if history is None and (lengths is not None or n_prompt is not None):
-        raise ValueError("process_logits: lengths and n_prompt belong to a history")
-    if (tree_tokens is None) != (tree_words is None):
-        raise ValueError("process_logits: give both tree_tokens and tree_words, or neither")
     if history is not None:
         if history.dtype != torch.int64:
             raise ValueError(f"process_logits: history must be int64, got {history.dtype}")
-        history, hist_stride = _row_stride(history, rows, 0, "process_logits: history")
-        hist_cap = history.shape[1]
+        history, hist_cap, hist_stride = _row_stride(history, rows, 0, "process_logits: history")
+        hist = history.data_ptr()
         if lengths is not None:
-            lengths = _index(lengths, 1 if lengths.numel() == 1 else rows, "process_logits: lengths")
-            len_stride = int(lengths.numel() != 1)
+            n = lengths.numel()
+            lengths = _index(lengths, 1 if n == 1 else rows, "process_logits: lengths")
+            lens, len_stride = lengths.data_ptr(), n != 1
         if n_prompt is not None:
-            n_prompt = _index(n_prompt, 1 if n_prompt.numel() == 1 else rows, "process_logits: n_prompt")
-            prompt_stride = int(n_prompt.numel() != 1)
-    if tree_tokens is not None:
+            n = n_prompt.numel()
+            n_prompt = _index(n_prompt, 1 if n == 1 else rows, "process_logits: n_prompt")
+            prompt, prompt_stride = n_prompt.data_ptr(), n != 1
+    elif lengths is not None or n_prompt is not None:
+        raise ValueError("process_logits: lengths and n_prompt belong to a history")
+    if tree_tokens is not None and tree_words is not None:
         n_tree = tree_tokens.numel()
         tree_tokens = _index(tree_tokens, n_tree, "process_logits: tree_tokens")
-        if (tree_words.dtype != torch.int32 or tree_words.dim() != 2 or tree_words.shape[0] != rows
-                or tree_words.shape[1] * 32 < n_tree or tree_words.stride(1) != 1):
+        ws = tree_words.shape
+        if (tree_words.dtype != torch.int32 or len(ws) != 2 or ws[0] != rows or ws[1] * 32 < n_tree
+                or tree_words.stride(1) != 1):
             raise ValueError(f"process_logits: tree_words must be int32, {rows} rows of at least {n_tree} bits")
         tree_words, tree_stride = _word_rows(tree_words)
+        toks, words = tree_tokens.data_ptr(), tree_words.data_ptr()
+    elif tree_tokens is not None or tree_words is not None:
+        raise ValueError("process_logits: give both tree_tokens and tree_words, or neither")
     if bias is not None:
         if bias.dtype != torch.float32:
             raise ValueError(f"process_logits: bias must be fp32, got {bias.dtype}")
-        bias, bias_stride = _row_stride(bias, rows, vocab, "process_logits: bias")
+        bias, _, bias_stride = _row_stride(bias, rows, vocab, "process_logits: bias")
+        bias_p = bias.data_ptr()
     if mask_words is not None:
         if mask_words.dtype != torch.int32:
             raise ValueError(f"process_logits: mask_words must be int32, got {mask_words.dtype}")
-        mask_words, mask_stride = _row_stride(mask_words, rows, (vocab + 31) // 32, "process_logits: mask_words")
-    out2 = None
+        mask_words, _, mask_stride = _row_stride(mask_words, rows, (vocab + 31) // 32, "process_logits: mask_words")
+        mask_p = mask_words.data_ptr()
+    out_p = out_code = out_stride = 0
     if out is not None:
         if out_dtype not in (None, out.dtype):
             raise ValueError(f"process_logits: out is {out.dtype}, out_dtype {out_dtype}")
         if out.numel() != rows * vocab or out.shape[-1] != vocab:
             raise ValueError(f"process_logits: out must be {rows} rows of {vocab}, got {list(out.shape)}")
         out2 = out.view(-1, vocab)
-        if out2.stride(1) != 1:
+        out_stride, col = out2.stride()
+        if col != 1:
             raise ValueError("process_logits: out rows must be contiguous")
+        out_p, out_code = out2.data_ptr(), _DT3.get(out.dtype)
     elif return_logits:
-        out = torch.empty(shape, dtype=out_dtype or logits.dtype, device=dev)
-        out2 = out if len(shape) == 2 else out.view(-1, vocab)
+        out = logits.new_empty(shape) if out_dtype is None else logits.new_empty(shape, dtype=out_dtype)
+        out_p, out_code, out_stride = out.data_ptr(), _DT3.get(out.dtype), vocab
+    if out_code is None:
+        raise NotImplementedError(f"process_logits: bf16, fp16 or fp32 output, got {out.dtype}")
     tokens = torch.empty(shape[:-1], dtype=torch.int64, device=dev)
-    if out2 is not None and out2.dtype not in _DT3:
-        raise NotImplementedError(f"process_logits: bf16, fp16 or fp32 output, got {out2.dtype}")
     if not (repetition > 0 and presence == presence and frequency == frequency):
         raise ValueError("process_logits: repetition must be > 0 and no penalty NaN")
     if repetition == 1.0 and presence == 0.0 and frequency == 0.0:
         hist_cap = n_tree = 0                    # nothing depends on the counts
-    _call("process_logits", dev, 1, logits.data_ptr(), _ptr(history), _ptr(lengths), _ptr(n_prompt), _ptr(bias),
-          _ptr(mask_words), _ptr(tree_tokens), _ptr(tree_words), _ptr(out2), tokens.data_ptr(), _ptr(status),
-          logits.stride(0) if rows > 1 else vocab, rows, vocab, hist_stride, hist_cap, len_stride, prompt_stride,
-          bias_stride, mask_stride, tree_stride, (out2.stride(0) if rows > 1 else vocab) if out2 is not None else 0,
-          n_tree, _DT3[logits.dtype], _DT3[out2.dtype] if out2 is not None else 0, repetition, presence, frequency)
+    if rows == 1:                                # one row's stride says nothing
+        row_stride = out_stride = vocab
+    _process_logits(dev, logits.data_ptr(), hist, lens, prompt, bias_p, mask_p, toks, words, out_p, tokens.data_ptr(),
+                    0 if status is None else status.data_ptr(), row_stride, rows, vocab, hist_stride, hist_cap,
+                    len_stride, prompt_stride, bias_stride, mask_stride, tree_stride, out_stride, n_tree, code,
+                    out_code, repetition, presence, frequency)
     return out, tokens
