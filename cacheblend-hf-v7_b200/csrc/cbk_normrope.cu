@@ -8,22 +8,29 @@
 // with (c, s) = table[p][i]; dimensions from R on pass through.  Q goes to
 // q_out[j], K to k_cache[r], V unchanged to v_cache[r].
 //
-// HBM-bound: every byte is read and written once.  A lane owns 8 consecutive
-// elements (16 bytes) of a head, LPH = D / 8 rounded up to a power of two lanes
-// make a head, a warp pass takes 32 / LPH heads, and a warp issues kUnroll
-// passes' loads before any arithmetic.  The sum of squares is a butterfly within
-// the head's lanes; the pair partner of the split layout lies R / 16 lanes away
-// (R is a multiple of 16), so a shuffle brings it.  Everything is held in fp32;
-// CBK_ROPE_REF adds the 16-bit roundings of the HF modules (the normalised value
-// before and after its weight, cos and sin, each product and the sum), so the
-// result has their bits; CBK_ROPE_FP32 rounds once, at the store.
-#include "cbk_common.cuh"
+// HBM-bound: every byte is read and written once.  A lane owns four pairs of a head
+// (8 elements: two 8-byte pieces half a rotation apart, or one 16-byte piece of
+// interleaved pairs), so both halves of a pair meet in its registers; LPH = D / 8
+// rounded up to a power of two lanes make a head and a warp pass takes 32 / LPH
+// heads, kNrUnroll passes' loads in flight.  The sum of squares is a butterfly
+// within the head's lanes.  A warp takes all heads of a token (several warps share
+// one when there are few tokens), so cos, sin and the weights are read and
+// multiplied together once per token: with wc = w c and ws = w s, and r the root,
+//   (z_a, z_b) = ((x_a wc_a - x_b ws_b) r, (x_b wc_b + x_a ws_a) r)
+// in packed fp32 pairs.  Everything is fp32 and rounded once at the store
+// (CBK_ROPE_FP32), or, in CBK_ROPE_REF, rounded to 16 bits where the HF modules do
+// (the normalised value before and after its weight, cos and sin, each product and
+// the sum) with packed 16-bit arithmetic, so the result has their bits.
+#include <algorithm>
+
+#include "cbk_attn_common.cuh"
 
 namespace cbk {
 
 constexpr int kNrThreads = 256;
 constexpr int kNrWarps = kNrThreads / 32;
 constexpr int kNrUnroll = 4;
+constexpr int64_t kNrFill = 148 * 32;        // warps that fill the GPU
 
 struct NormRopeParams {
   const uint16_t *q, *k, *v, *qw, *kw;
@@ -33,136 +40,201 @@ struct NormRopeParams {
   uint16_t *q_out, *k_cache, *v_cache;
   int32_t* status;
   int64_t n, table_rows, cap, kv_stride;
-  int n_q, n_kv, dim, rotary, chunks;   // chunks: warps per token
+  int n_q, n_kv, dim, rotary, parts;    // parts: warps per token
   float eps, inv_dim;
+};
+
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// a packed 16-bit pair as an fp32 pair
+template <int DT>
+__device__ __forceinline__ uint64_t widen(uint32_t w) {
+  return pk_f2(Elem<DT>::to_f(static_cast<uint16_t>(w)), Elem<DT>::to_f(static_cast<uint16_t>(w >> 16)));
+}
+template <int DT>
+__device__ __forceinline__ uint32_t narrow(uint64_t f2) {
+  float lo, hi;
+  upk_f2(f2, lo, hi);
+  return Pk<DT>::cvt(lo, hi);
+}
+
+// a lane's four pairs: a[0], a[1] hold the first elements of pairs (0, 1) and (2, 3), b the second ones
+struct Four {
+  uint32_t a[2], b[2];
 };
 
 template <int DT, int LPH, bool REF, bool PAIRS>
 __global__ void __launch_bounds__(kNrThreads)
 norm_rope_scatter_kernel(const NormRopeParams p) {
-  using E = Elem<DT>;
   constexpr int kHeads = 32 / LPH;          // heads per warp pass
   constexpr unsigned kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
   const int64_t gw = static_cast<int64_t>(blockIdx.x) * kNrWarps + (threadIdx.x >> 5);
-  const int64_t j = gw / p.chunks;
+  const int64_t j = gw / p.parts;
   if (j >= p.n) return;
-  const int part = static_cast<int>(gw - j * p.chunks);
+  const int part = static_cast<int>(gw - j * p.parts);
   const int64_t pos = p.pos[j], row = p.rows[j];
-  const int l = lane & (LPH - 1), e0 = 8 * l;
-  const int n_heads = p.n_q + 2 * p.n_kv;
-  const int head0 = part * kNrUnroll * kHeads + lane / LPH;
+  // passes over the heads of Q, then of K, then over V's row in 512-byte pieces
+  const int pq = (p.n_q + kHeads - 1) / kHeads, pk = (p.n_kv + kHeads - 1) / kHeads;
+  const int v_cols = p.n_kv * p.dim, pv = (v_cols + 255) / 256, all = pq + pk + pv;
+  const int first = all * part / p.parts, last = all * (part + 1) / p.parts;
+  const int l = lane & (LPH - 1), half = p.rotary / 2;
+  const bool live = 8 * l < p.dim, turns = 8 * l < p.rotary;
+  // the lane's elements of a head: [ea, ea + 4) and [eb, eb + 4)
+  const int ea = PAIRS || !turns ? 8 * l : 4 * l;
+  const int eb = PAIRS || !turns ? 8 * l + 4 : half + 4 * l;
 
-  uint4 raw[kNrUnroll];
-#pragma unroll
-  for (int u = 0; u < kNrUnroll; ++u) {
-    const int h = head0 + u * kHeads;
-    raw[u] = make_uint4(0, 0, 0, 0);
-    if (h < n_heads && e0 < p.dim) {
-      const uint16_t* src;
-      if (h < p.n_q) src = p.q + j * p.qs + static_cast<int64_t>(h) * p.dim;
-      else if (h < p.n_q + p.n_kv) src = p.k + j * p.ks + static_cast<int64_t>(h - p.n_q) * p.dim;
-      else src = p.v + j * p.vs + static_cast<int64_t>(h - p.n_q - p.n_kv) * p.dim;
-      raw[u] = ld_stream(src + e0);
-    }
-  }
   if (row == -1) return;                    // padding token: nothing of it is written
   if (pos < 0 || pos >= p.table_rows || row < 0 || row >= p.cap) {
     if (part == 0 && lane == 0) report(p.status, CBK_STATUS_BAD_INDEX);
     return;
   }
 
-  // cos / sin of the lane's elements: 8 pairs in the split layout, 4 interleaved
-  constexpr int kCs = PAIRS ? 4 : 8;
-  const bool turns = e0 < p.rotary;
-  const int half = p.rotary / 2;
-  float c[kCs], s[kCs];
-  int partner = lane;
-  {
-    const int i0 = PAIRS ? e0 / 2 : (e0 < half ? e0 : e0 - half);
-    const float4* t = p.table + (pos * half + i0) / 2;
-#pragma unroll
-    for (int i = 0; i < kCs / 2; ++i) {
-      const float4 cs = turns ? __ldg(t + i) : make_float4(1.f, 0.f, 1.f, 0.f);
-      c[2 * i] = cs.x;
-      s[2 * i] = cs.y;
-      c[2 * i + 1] = cs.z;
-      s[2 * i + 1] = cs.w;
+  auto load = [&](const uint16_t* head) {
+    Four x = {{0, 0}, {0, 0}};
+    if (PAIRS) {
+      const uint4 r = ld_stream(head + ea);
+      // interleaved: word i holds pair i
+      x.a[0] = __byte_perm(r.x, r.y, 0x5410);
+      x.b[0] = __byte_perm(r.x, r.y, 0x7632);
+      x.a[1] = __byte_perm(r.z, r.w, 0x5410);
+      x.b[1] = __byte_perm(r.z, r.w, 0x7632);
+    } else {
+      const uint2 ra = __ldcs(reinterpret_cast<const uint2*>(head + ea));
+      const uint2 rb = __ldcs(reinterpret_cast<const uint2*>(head + eb));
+      x.a[0] = ra.x;
+      x.a[1] = ra.y;
+      x.b[0] = rb.x;
+      x.b[1] = rb.y;
     }
-    if (!PAIRS && turns) partner = e0 < half ? lane + half / 8 : lane - half / 8;
-#pragma unroll
-    for (int i = 0; i < kCs; ++i) {
-      if (REF) {
-        c[i] = round16<DT>(c[i]);
-        s[i] = round16<DT>(s[i]);
-      }
-      if (!PAIRS && e0 < half) s[i] = -s[i];   // first of the pair: y_a c - y_b s
+    return x;
+  };
+  auto store = [&](uint16_t* head, const Four& x) {
+    if (PAIRS) {
+      st_vec(head + ea, make_uint4(__byte_perm(x.a[0], x.b[0], 0x5410), __byte_perm(x.a[0], x.b[0], 0x7632),
+                                   __byte_perm(x.a[1], x.b[1], 0x5410), __byte_perm(x.a[1], x.b[1], 0x7632)));
+    } else {
+      *reinterpret_cast<uint2*>(head + ea) = make_uint2(x.a[0], x.a[1]);
+      *reinterpret_cast<uint2*>(head + eb) = make_uint2(x.b[0], x.b[1]);
     }
-  }
-  const bool norm = p.qw != nullptr;
-  uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
-  if (norm && e0 < p.dim) {
-    wq = ld_vec(p.qw + e0);
-    wk = ld_vec(p.kw + e0);
-  }
+  };
 
+  if (first < pq + pk) {
+    // cos and sin of the lane's pairs (1, 0 where nothing turns)
+    float4 t0 = make_float4(1.f, 0.f, 1.f, 0.f), t1 = t0;
+    if (turns) {
+      const float4* t = p.table + (pos * half + 4 * l) / 2;
+      t0 = __ldg(t);
+      t1 = __ldg(t + 1);
+    }
+    const bool norm = p.qw != nullptr;
+    const uint64_t c[2] = {pk_f2(t0.x, t0.z), pk_f2(t1.x, t1.z)}, s[2] = {pk_f2(t0.y, t0.w), pk_f2(t1.y, t1.w)};
+    const uint32_t c16[2] = {narrow<DT>(c[0]), narrow<DT>(c[1])}, s16[2] = {narrow<DT>(s[0]), narrow<DT>(s[1])};
+
+#pragma unroll 1
+    for (int kv = 0; kv < 2; ++kv) {        // passes [from, to) over the heads of Q's row, then of K's
+      const uint16_t* src = kv ? p.k + j * p.ks : p.q + j * p.qs;
+      uint16_t* dst = kv ? p.k_cache + row * p.kv_stride : p.q_out + j * p.n_q * p.dim;
+      const uint16_t* weight = kv ? p.kw : p.qw;
+      const int n_heads = kv ? p.n_kv : p.n_q;
+      const int from = max(first - kv * pq, 0), to = min(last - kv * pq, kv ? pk : pq);
+      if (from >= to) continue;
+      Four w = {{0, 0}, {0, 0}};
+      if (norm && live) w = load(weight);
+      uint64_t ca[2], cb[2], sa[2], sb[2];
 #pragma unroll
-  for (int u = 0; u < kNrUnroll; ++u) {
-    const int h = head0 + u * kHeads;
-    const bool is_q = h < p.n_q, is_v = h >= p.n_q + p.n_kv;
-    const uint16_t* hx = reinterpret_cast<const uint16_t*>(&raw[u]);
-    float y[8];
+      for (int i = 0; i < 2; ++i) {
+        const uint64_t wa = norm ? widen<DT>(w.a[i]) : pk_f2(1.f, 1.f), wb = norm ? widen<DT>(w.b[i]) : pk_f2(1.f, 1.f);
+        ca[i] = mul_f2(wa, c[i]);
+        cb[i] = mul_f2(wb, c[i]);
+        sa[i] = mul_f2(wa, s[i]);
+        sb[i] = mul_f2(wb, s[i]) ^ 0x8000000080000000ull;      // z_a takes - x_b w_b s
+      }
+      for (int p0 = from; p0 < to; p0 += kNrUnroll) {
+        Four x[kNrUnroll];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = E::to_f(hx[e]);
-    if (norm) {
-      float ss = 0.f;
+        for (int u = 0; u < kNrUnroll; ++u) {
+          const int h = (p0 + u) * kHeads + lane / LPH;
+          x[u] = {{0, 0}, {0, 0}};
+          if (p0 + u < to && h < n_heads && live) x[u] = load(src + static_cast<int64_t>(h) * p.dim);
+        }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
+        for (int u = 0; u < kNrUnroll; ++u) {
+          if (p0 + u >= to) break;
+          const int h = (p0 + u) * kHeads + lane / LPH;
+          uint64_t a[2], b[2];
 #pragma unroll
-      for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(kAll, ss, o);
-      const float r = rsqrtf(fmaf(ss, p.inv_dim, p.eps));
-      const uint4 w4 = is_q ? wq : wk;
-      const uint16_t* hw = reinterpret_cast<const uint16_t*>(&w4);
+          for (int i = 0; i < 2; ++i) {
+            a[i] = widen<DT>(x[u].a[i]);
+            b[i] = widen<DT>(x[u].b[i]);
+          }
+          float r = 1.f;
+          if (norm) {
+            uint64_t q = mul_f2(a[0], a[0]);
+            q = fma_f2(b[0], b[0], q);
+            q = fma_f2(a[1], a[1], q);
+            q = fma_f2(b[1], b[1], q);
+            float q0, q1;
+            upk_f2(q, q0, q1);
+            float ss = q0 + q1;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float w = E::to_f(hw[e]);
-        y[e] = REF ? round16<DT>(w * round16<DT>(y[e] * r)) : y[e] * r * w;
+            for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(kAll, ss, o);
+            r = rsqrtf(fmaf(ss, p.inv_dim, p.eps));
+          }
+          const uint64_t rr = pk_f2(r, r);
+          Four z;
+          if (REF) {
+            Four y = x[u];
+            if (norm) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                y.a[i] = Pk<DT>::mul(w.a[i], narrow<DT>(mul_f2(a[i], rr)));
+                y.b[i] = Pk<DT>::mul(w.b[i], narrow<DT>(mul_f2(b[i], rr)));
+              }
+            }
+            z = y;
+            if (turns) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                z.a[i] = Pk<DT>::sub(Pk<DT>::mul(y.a[i], c16[i]), Pk<DT>::mul(y.b[i], s16[i]));
+                z.b[i] = Pk<DT>::add(Pk<DT>::mul(y.b[i], c16[i]), Pk<DT>::mul(y.a[i], s16[i]));
+              }
+            }
+          } else if (turns || norm) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              // (where nothing turns only the weight: 0 * x would spread a neighbour's infinity)
+              const uint64_t za = turns ? fma_f2(a[i], ca[i], mul_f2(b[i], sb[i])) : mul_f2(a[i], ca[i]);
+              const uint64_t zb = turns ? fma_f2(b[i], cb[i], mul_f2(a[i], sa[i])) : mul_f2(b[i], cb[i]);
+              z.a[i] = narrow<DT>(mul_f2(za, rr));
+              z.b[i] = narrow<DT>(mul_f2(zb, rr));
+            }
+          } else {
+            z = x[u];
+          }
+          if (h < n_heads && live) store(dst + static_cast<int64_t>(h) * p.dim, z);
+        }
       }
     }
-    float z[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (PAIRS) {
-        const float other = y[e ^ 1], sn = (e & 1) ? s[e / 2] : -s[e / 2];
-        z[e] = REF ? round16<DT>(y[e] * c[e / 2]) + round16<DT>(other * sn) : fmaf(y[e], c[e / 2], other * sn);
-      } else {
-        const float other = __shfl_sync(kAll, y[e], partner);
-        z[e] = REF ? round16<DT>(y[e] * c[e % kCs]) + round16<DT>(other * s[e % kCs])
-                   : fmaf(y[e], c[e % kCs], other * s[e % kCs]);
-      }
-    }
-    if (h >= n_heads || e0 >= p.dim) continue;
-    uint4 o = raw[u];
-    if (!is_v) {
-      uint32_t* w = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = turns ? Pk<DT>::cvt(z[2 * e], z[2 * e + 1]) : Pk<DT>::cvt(y[2 * e], y[2 * e + 1]);
-    }
-    uint16_t* dst;
-    if (is_q) dst = p.q_out + (j * p.n_q + h) * p.dim;
-    else if (!is_v) dst = p.k_cache + row * p.kv_stride + static_cast<int64_t>(h - p.n_q) * p.dim;
-    else dst = p.v_cache + row * p.kv_stride + static_cast<int64_t>(h - p.n_q - p.n_kv) * p.dim;
-    st_vec(dst + e0, o);
+  }
+  for (int i = max(first - pq - pk, 0); i < last - pq - pk; ++i) {
+    const int e = i * 256 + lane * 8;
+    if (e < v_cols) st_vec(p.v_cache + row * p.kv_stride + e, ld_stream(p.v + j * p.vs + e));
   }
 }
 
 template <int DT, int LPH>
 static int launch_norm_rope(NormRopeParams& p, int interleaved, int mode, cudaStream_t st) {
   constexpr int kHeads = 32 / LPH;
-  const int passes = (p.n_q + 2 * p.n_kv + kHeads - 1) / kHeads;
-  p.chunks = (passes + kNrUnroll - 1) / kNrUnroll;
-  const int64_t blocks = (p.n * p.chunks + kNrWarps - 1) / kNrWarps;
+  const int passes = (p.n_q + kHeads - 1) / kHeads + (p.n_kv + kHeads - 1) / kHeads + (p.n_kv * p.dim + 255) / 256;
+  // a warp per token once that fills the GPU (32 warps on each of ~148 SMs), else the
+  // passes of a token over as many warps as it takes
+  const int64_t want = (kNrFill + p.n - 1) / p.n;
+  p.parts = static_cast<int>(std::min<int64_t>(passes, std::max<int64_t>(1, want)));
+  const int64_t blocks = (p.n * p.parts + kNrWarps - 1) / kNrWarps;
   if (blocks > 0x7fffffff) return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: too many tokens");
   const unsigned g = static_cast<unsigned>(blocks);
   if (mode == CBK_ROPE_REF) {
