@@ -11,11 +11,14 @@
 // HBM-bound: every byte is read and written once.  A lane owns four pairs of a head
 // (8 elements: two 8-byte pieces half a rotation apart, or one 16-byte piece of
 // interleaved pairs), so both halves of a pair meet in its registers; LPH = D / 8
-// rounded up to a power of two lanes make a head and a warp pass takes 32 / LPH
-// heads, kNrUnroll passes' loads in flight.  The sum of squares is a butterfly
-// within the head's lanes.  A warp takes all heads of a token (several warps share
-// one when there are few tokens), so cos, sin and the weights are read and
-// multiplied together once per token: with wc = w c and ws = w s, and r the root,
+// rounded up to a power of two lanes make a head, a warp pass takes 32 / LPH heads
+// and kNrUnroll passes are a chunk.  Sources arrive by bulk copies into kNrSlots
+// chunks of shared memory per warp, so the bytes in flight cost no registers
+// (loads into registers: 171 us for 32768 tokens of 32 + 8 heads of 128, bound by
+// the loads' latency at the occupancy the registers left).  The sum of squares is
+// a butterfly within the head's lanes.  A warp takes all heads of a token (several
+// warps share one when there are few tokens), so cos, sin and the weights are read
+// and multiplied together once per token: with wc = w c, ws = w s and r the root,
 //   (z_a, z_b) = ((x_a wc_a - x_b ws_b) r, (x_b wc_b + x_a ws_a) r)
 // in packed fp32 pairs.  Everything is fp32 and rounded once at the store
 // (CBK_ROPE_FP32), or, in CBK_ROPE_REF, rounded to 16 bits where the HF modules do
@@ -27,10 +30,15 @@
 
 namespace cbk {
 
+int ensure_smem_attr(const void* func, int bytes);   // cbk_api.cu
+
 constexpr int kNrThreads = 256;
 constexpr int kNrWarps = kNrThreads / 32;
-constexpr int kNrUnroll = 4;
-constexpr int64_t kNrFill = 148 * 32;        // warps that fill the GPU
+constexpr int kNrUnroll = 4;                 // warp passes of a chunk
+constexpr int kNrSlots = 4;                  // chunks in flight per warp
+constexpr int kNrSlotBytes = kNrUnroll * 512;
+constexpr int kNrSmem = kNrWarps * kNrSlots * kNrSlotBytes;
+constexpr int64_t kNrFill = 148 * 24;        // warps that fill the GPU
 
 struct NormRopeParams {
   const uint16_t *q, *k, *v, *qw, *kw;
@@ -66,45 +74,87 @@ struct Four {
   uint32_t a[2], b[2];
 };
 
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
 template <int DT, int LPH, bool REF, bool PAIRS>
-__global__ void __launch_bounds__(kNrThreads)
+__global__ void __launch_bounds__(kNrThreads, 3)
 norm_rope_scatter_kernel(const NormRopeParams p) {
-  constexpr int kHeads = 32 / LPH;          // heads per warp pass
+  constexpr int kHeads = 32 / LPH;                   // heads per warp pass
+  constexpr int kChunk = kNrUnroll * kHeads;         // heads per chunk
   constexpr unsigned kAll = 0xffffffffu;
-  const int lane = threadIdx.x & 31;
-  const int64_t gw = static_cast<int64_t>(blockIdx.x) * kNrWarps + (threadIdx.x >> 5);
+  extern __shared__ __align__(128) uint8_t s_rows[];
+  __shared__ uint64_t s_bar[kNrWarps][kNrSlots];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t gw = static_cast<int64_t>(blockIdx.x) * kNrWarps + warp;
   const int64_t j = gw / p.parts;
   if (j >= p.n) return;
   const int part = static_cast<int>(gw - j * p.parts);
-  const int64_t pos = p.pos[j], row = p.rows[j];
-  // passes over the heads of Q, then of K, then over V's row in 512-byte pieces
-  const int pq = (p.n_q + kHeads - 1) / kHeads, pk = (p.n_kv + kHeads - 1) / kHeads;
-  const int v_cols = p.n_kv * p.dim, pv = (v_cols + 255) / 256, all = pq + pk + pv;
+  // chunks over the heads of Q, then of K, then over V's row in pieces of a slot
+  constexpr int kVPiece = kNrSlotBytes / 2;
+  const int v_cols = p.n_kv * p.dim;
+  const int cq = (p.n_q + kChunk - 1) / kChunk, ck = (p.n_kv + kChunk - 1) / kChunk;
+  const int cv = (v_cols + kVPiece - 1) / kVPiece, all = cq + ck + cv;
   const int first = all * part / p.parts, last = all * (part + 1) / p.parts;
+
+  const uint32_t bar0 = smem_u32(&s_bar[warp][0]);
+  uint8_t* slots = s_rows + warp * kNrSlots * kNrSlotBytes;
+  auto fetch = [&](int c) {                          // chunk c into slot (c - first) % kNrSlots; one lane
+    const uint16_t* src;
+    int cols;
+    if (c < cq) {
+      src = p.q + j * p.qs + static_cast<int64_t>(c) * kChunk * p.dim;
+      cols = min(kChunk, p.n_q - c * kChunk) * p.dim;
+    } else if (c < cq + ck) {
+      src = p.k + j * p.ks + static_cast<int64_t>(c - cq) * kChunk * p.dim;
+      cols = min(kChunk, p.n_kv - (c - cq) * kChunk) * p.dim;
+    } else {
+      src = p.v + j * p.vs + static_cast<int64_t>(c - cq - ck) * kVPiece;
+      cols = min(kVPiece, v_cols - (c - cq - ck) * kVPiece);
+    }
+    const int slot = (c - first) % kNrSlots;
+    mbar_expect_tx(bar0 + 8 * slot, cols * 2);
+    bulk_load(smem_u32(slots + slot * kNrSlotBytes), src, cols * 2, bar0 + 8 * slot);
+  };
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kNrSlots; ++i) mbar_init(bar0 + 8 * i, 1);
+    fence_barrier_init();
+    for (int c = first; c < min(last, first + kNrSlots); ++c) fetch(c);
+  }
+  __syncwarp();
+  const int64_t pos = p.pos[j], row = p.rows[j];
+  bool failed = false;
+  auto landed = [&](int c) {
+    if (!__all_sync(kAll, mbar_wait(bar0 + 8 * ((c - first) % kNrSlots), ((c - first) / kNrSlots) & 1))) failed = true;
+    return !failed;
+  };
+  const bool bad = row != -1 && (pos < 0 || pos >= p.table_rows || row < 0 || row >= p.cap);
+  if (row == -1 || bad) {                            // padding token, or one that is skipped
+    if (bad && part == 0 && lane == 0) report(p.status, CBK_STATUS_BAD_INDEX);
+    for (int c = first; c < min(last, first + kNrSlots); ++c) landed(c);      // its copies end before the CTA does
+    if (failed) report(p.status, CBK_STATUS_TIMEOUT);
+    return;
+  }
+
   const int l = lane & (LPH - 1), half = p.rotary / 2;
   const bool live = 8 * l < p.dim, turns = 8 * l < p.rotary;
   // the lane's elements of a head: [ea, ea + 4) and [eb, eb + 4)
   const int ea = PAIRS || !turns ? 8 * l : 4 * l;
   const int eb = PAIRS || !turns ? 8 * l + 4 : half + 4 * l;
-
-  if (row == -1) return;                    // padding token: nothing of it is written
-  if (pos < 0 || pos >= p.table_rows || row < 0 || row >= p.cap) {
-    if (part == 0 && lane == 0) report(p.status, CBK_STATUS_BAD_INDEX);
-    return;
-  }
-
   auto load = [&](const uint16_t* head) {
-    Four x = {{0, 0}, {0, 0}};
+    Four x;
     if (PAIRS) {
-      const uint4 r = ld_stream(head + ea);
+      const uint4 r = *reinterpret_cast<const uint4*>(head + ea);
       // interleaved: word i holds pair i
       x.a[0] = __byte_perm(r.x, r.y, 0x5410);
       x.b[0] = __byte_perm(r.x, r.y, 0x7632);
       x.a[1] = __byte_perm(r.z, r.w, 0x5410);
       x.b[1] = __byte_perm(r.z, r.w, 0x7632);
     } else {
-      const uint2 ra = __ldcs(reinterpret_cast<const uint2*>(head + ea));
-      const uint2 rb = __ldcs(reinterpret_cast<const uint2*>(head + eb));
+      const uint2 ra = *reinterpret_cast<const uint2*>(head + ea), rb = *reinterpret_cast<const uint2*>(head + eb);
       x.a[0] = ra.x;
       x.a[1] = ra.y;
       x.b[0] = rb.x;
@@ -122,7 +172,8 @@ norm_rope_scatter_kernel(const NormRopeParams p) {
     }
   };
 
-  if (first < pq + pk) {
+  int c_now = first;                                 // chunks taken so far
+  if (first < cq + ck) {
     // cos and sin of the lane's pairs (1, 0 where nothing turns)
     float4 t0 = make_float4(1.f, 0.f, 1.f, 0.f), t1 = t0;
     if (turns) {
@@ -135,13 +186,12 @@ norm_rope_scatter_kernel(const NormRopeParams p) {
     const uint32_t c16[2] = {narrow<DT>(c[0]), narrow<DT>(c[1])}, s16[2] = {narrow<DT>(s[0]), narrow<DT>(s[1])};
 
 #pragma unroll 1
-    for (int kv = 0; kv < 2; ++kv) {        // passes [from, to) over the heads of Q's row, then of K's
-      const uint16_t* src = kv ? p.k + j * p.ks : p.q + j * p.qs;
+    for (int kv = 0; kv < 2; ++kv) {                 // the chunks of Q's row, then of K's
+      const int end = min(last, kv ? cq + ck : cq);
+      if (c_now >= end) continue;
       uint16_t* dst = kv ? p.k_cache + row * p.kv_stride : p.q_out + j * p.n_q * p.dim;
       const uint16_t* weight = kv ? p.kw : p.qw;
       const int n_heads = kv ? p.n_kv : p.n_q;
-      const int from = max(first - kv * pq, 0), to = min(last - kv * pq, kv ? pk : pq);
-      if (from >= to) continue;
       Four w = {{0, 0}, {0, 0}};
       if (norm && live) w = load(weight);
       uint64_t ca[2], cb[2], sa[2], sb[2];
@@ -153,18 +203,21 @@ norm_rope_scatter_kernel(const NormRopeParams p) {
         sa[i] = mul_f2(wa, s[i]);
         sb[i] = mul_f2(wb, s[i]) ^ 0x8000000080000000ull;      // z_a takes - x_b w_b s
       }
-      for (int p0 = from; p0 < to; p0 += kNrUnroll) {
+      for (; c_now < end; ++c_now) {
+        if (!landed(c_now)) break;
+        const uint16_t* chunk = reinterpret_cast<const uint16_t*>(slots + (c_now - first) % kNrSlots * kNrSlotBytes);
+        const int h0 = (c_now - (kv ? cq : 0)) * kChunk + lane / LPH;
         Four x[kNrUnroll];
 #pragma unroll
         for (int u = 0; u < kNrUnroll; ++u) {
-          const int h = (p0 + u) * kHeads + lane / LPH;
           x[u] = {{0, 0}, {0, 0}};
-          if (p0 + u < to && h < n_heads && live) x[u] = load(src + static_cast<int64_t>(h) * p.dim);
+          if (h0 + u * kHeads < n_heads && live) x[u] = load(chunk + (u * kHeads + lane / LPH) * p.dim);
         }
+        __syncwarp();                                // the slot is read
+        if (lane == 0 && c_now + kNrSlots < last) fetch(c_now + kNrSlots);
 #pragma unroll
         for (int u = 0; u < kNrUnroll; ++u) {
-          if (p0 + u >= to) break;
-          const int h = (p0 + u) * kHeads + lane / LPH;
+          const int h = h0 + u * kHeads;
           uint64_t a[2], b[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -220,30 +273,46 @@ norm_rope_scatter_kernel(const NormRopeParams p) {
       }
     }
   }
-  for (int i = max(first - pq - pk, 0); i < last - pq - pk; ++i) {
-    const int e = i * 256 + lane * 8;
-    if (e < v_cols) st_vec(p.v_cache + row * p.kv_stride + e, ld_stream(p.v + j * p.vs + e));
+  for (; c_now < last && !failed; ++c_now) {
+    if (!landed(c_now)) break;
+    const int e0 = (c_now - cq - ck) * kVPiece;
+    const uint16_t* chunk = reinterpret_cast<const uint16_t*>(slots + (c_now - first) % kNrSlots * kNrSlotBytes);
+    uint4 x[kVPiece / 256];
+#pragma unroll
+    for (int i = 0; i < kVPiece / 256; ++i) x[i] = ld_vec(chunk + i * 256 + lane * 8);
+    __syncwarp();
+    if (lane == 0 && c_now + kNrSlots < last) fetch(c_now + kNrSlots);
+#pragma unroll
+    for (int i = 0; i < kVPiece / 256; ++i) {
+      const int e = e0 + i * 256 + lane * 8;
+      if (e < v_cols) st_vec(p.v_cache + row * p.kv_stride + e, x[i]);
+    }
+  }
+  if (failed) {
+    for (int c = c_now; c < min(last, c_now + kNrSlots); ++c) landed(c);
+    report(p.status, CBK_STATUS_TIMEOUT);
   }
 }
 
 template <int DT, int LPH>
 static int launch_norm_rope(NormRopeParams& p, int interleaved, int mode, cudaStream_t st) {
   constexpr int kHeads = 32 / LPH;
-  const int passes = (p.n_q + kHeads - 1) / kHeads + (p.n_kv + kHeads - 1) / kHeads + (p.n_kv * p.dim + 255) / 256;
-  // a warp per token once that fills the GPU (32 warps on each of ~148 SMs), else the
-  // passes of a token over as many warps as it takes
+  constexpr int kChunk = kNrUnroll * kHeads, kVPiece = kNrSlotBytes / 2;
+  const int chunks = (p.n_q + kChunk - 1) / kChunk + (p.n_kv + kChunk - 1) / kChunk +
+                     (p.n_kv * p.dim + kVPiece - 1) / kVPiece;
+  // a warp per token once that fills the GPU, else the chunks of a token over as many
+  // warps as it takes
   const int64_t want = (kNrFill + p.n - 1) / p.n;
-  p.parts = static_cast<int>(std::min<int64_t>(passes, std::max<int64_t>(1, want)));
+  p.parts = static_cast<int>(std::min<int64_t>(chunks, std::max<int64_t>(1, want)));
   const int64_t blocks = (p.n * p.parts + kNrWarps - 1) / kNrWarps;
   if (blocks > 0x7fffffff) return set_error(CBK_ERR_INVALID, "cbk_norm_rope_scatter: too many tokens");
-  const unsigned g = static_cast<unsigned>(blocks);
-  if (mode == CBK_ROPE_REF) {
-    if (interleaved) norm_rope_scatter_kernel<DT, LPH, true, true><<<g, kNrThreads, 0, st>>>(p);
-    else norm_rope_scatter_kernel<DT, LPH, true, false><<<g, kNrThreads, 0, st>>>(p);
-  } else {
-    if (interleaved) norm_rope_scatter_kernel<DT, LPH, false, true><<<g, kNrThreads, 0, st>>>(p);
-    else norm_rope_scatter_kernel<DT, LPH, false, false><<<g, kNrThreads, 0, st>>>(p);
-  }
+  void (*kern)(const NormRopeParams) =
+      mode == CBK_ROPE_REF ? (interleaved ? norm_rope_scatter_kernel<DT, LPH, true, true>
+                                          : norm_rope_scatter_kernel<DT, LPH, true, false>)
+                           : (interleaved ? norm_rope_scatter_kernel<DT, LPH, false, true>
+                                          : norm_rope_scatter_kernel<DT, LPH, false, false>);
+  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kNrSmem)) return rc;
+  kern<<<static_cast<unsigned>(blocks), kNrThreads, kNrSmem, st>>>(p);
   return check_launch("norm_rope_scatter_kernel");
 }
 
