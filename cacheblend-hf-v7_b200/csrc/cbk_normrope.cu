@@ -15,7 +15,9 @@
 // and kNrUnroll passes are a chunk.  Sources arrive by bulk copies into kNrSlots
 // chunks of shared memory per warp, so the bytes in flight cost no registers
 // (loads into registers: 171 us for 32768 tokens of 32 + 8 heads of 128, bound by
-// the loads' latency at the occupancy the registers left).  The sum of squares is
+// the loads' latency at the occupancy the registers left; this way 149 us = 5.5 TB/s,
+// 0.84 of measured HBM).  Chunks of 4 passes took 146 us there but 3.8 instead of
+// 3.1 us for one token; 2, 4 or 8 slots, 4 or 8 CTAs of 256 threads were slower.  The sum of squares is
 // a butterfly within the head's lanes.  A warp takes all heads of a token (several
 // warps share one when there are few tokens), so cos, sin and the weights are read
 // and multiplied together once per token: with wc = w c, ws = w s and r the root,
@@ -32,13 +34,13 @@ namespace cbk {
 
 int ensure_smem_attr(const void* func, int bytes);   // cbk_api.cu
 
-constexpr int kNrThreads = 256;
+constexpr int kNrThreads = 128;
 constexpr int kNrWarps = kNrThreads / 32;
-constexpr int kNrUnroll = 4;                 // warp passes of a chunk
-constexpr int kNrSlots = 4;                  // chunks in flight per warp
+constexpr int kNrUnroll = 2;                 // warp passes of a chunk
+constexpr int kNrSlots = 3;                  // chunks in flight per warp
 constexpr int kNrSlotBytes = kNrUnroll * 512;
 constexpr int kNrSmem = kNrWarps * kNrSlots * kNrSlotBytes;
-constexpr int64_t kNrFill = 148 * 24;        // warps that fill the GPU
+constexpr int64_t kNrFill = 148 * 24;        // warps that fill the GPU: six CTAs of four on each of 148 SMs
 
 struct NormRopeParams {
   const uint16_t *q, *k, *v, *qw, *kw;
@@ -80,7 +82,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 
 template <int DT, int LPH, bool REF, bool PAIRS>
-__global__ void __launch_bounds__(kNrThreads, 3)
+__global__ void __launch_bounds__(kNrThreads, 6)
 norm_rope_scatter_kernel(const NormRopeParams p) {
   constexpr int kHeads = 32 / LPH;                   // heads per warp pass
   constexpr int kChunk = kNrUnroll * kHeads;         // heads per chunk
