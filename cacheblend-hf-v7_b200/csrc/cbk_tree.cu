@@ -16,8 +16,7 @@
 // TMEM and a softmax warpgroup of its own, so one slot's softmax runs while the
 // tensor core works for the other.  With two Q tiles, slot t is tile t and every
 // key tile goes to both; with one Q tile both slots hold that tile and take the
-// key tiles in turn, each with its own running max, sum and O (two partial
-// results for the merge).  Unit u of a CTA (slot u & 1) is then key tile u >> 1 or
+// key tiles in turn, each with its own running max, sum and O, joined at the end.  Unit u of a CTA (slot u & 1) is then key tile u >> 1 or
 // u, and the MMA warp's order is the same for both: O += P(u) V(u), then
 // S(u + 2) = Q K(u + 2)^T, which overwrites P(u) after the PV that reads it.
 //
@@ -38,6 +37,7 @@
 // Every wait is bounded; on timeout the kernel sets CBK_STATUS_TIMEOUT, drains its
 // copies and MMAs, frees TMEM and returns.
 #include <algorithm>
+#include <type_traits>
 
 #include "cbk_attn_common.cuh"
 
@@ -78,8 +78,10 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeParams& p) {
   s.n_tiles = static_cast<int>((s.n_keys + kBN - 1) / kBN);
   return s;
 }
+// the first n_tiles % n_splits splits take one tile more than the others
 __device__ __forceinline__ int split_start(int n_tiles, int n_splits, int s) {
-  return static_cast<int>(static_cast<int64_t>(n_tiles) * s / n_splits);
+  const int each = n_tiles / n_splits;
+  return s * each + min(s, n_tiles - each * n_splits);
 }
 
 // 32 visibility bits of the keys at tree offsets [off, off + 32) of a node: offsets
@@ -441,21 +443,55 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(PFULL + t));
       }
+      // One Q tile: both slots' O lie in the same TMEM lanes, so the two warps of a
+      // row join them, each for half of the head dimensions.  Two: every slot is its
+      // tile's result.
+      const bool other = !two && n > 1;                      // the other slot holds a part of this row
       if (!failed && !wait_all(bar(ODONE + t), 0)) failed = true;
+      if (!failed && other && !wait_all(bar(ODONE + (t ^ 1)), 0)) failed = true;
+      float w_own = 1.f, w_other = 0.f;
+      if (other) {
+        // (every MMA is complete: Q's room is free for the rows' (max, sum))
+        float2* ml = reinterpret_cast<float2*>(sbase);
+        ml[t * kBM + row] = make_float2(m_used, l_sum);
+        // the active warps of both slots (a warp that failed arrives too)
+        asm volatile("bar.sync 1, %0;" ::"r"(2 * 32 * ((n_rows + 31) / 32)) : "memory");
+        const float2 x = ml[(t ^ 1) * kBM + row];
+        // a slot without a visible key has l = 0 and weight 0; its O is 0
+        const float m = fmaxf(l_sum != 0.f ? m_used : -INFINITY, x.y != 0.f ? x.x : -INFINITY);
+        w_own = l_sum != 0.f ? ex2(m_used - m) : 0.f;
+        w_other = x.y != 0.f ? ex2(x.x - m) : 0.f;
+        l_sum = (l_sum != 0.f ? w_own * l_sum : 0.f) + (x.y != 0.f ? w_other * x.y : 0.f);
+        m_used = m;
+      }
       if (!failed) {
         tc_fence_after();
-        const int64_t slot = ((static_cast<int64_t>(kvh) * p.n_pairs + pair) * p.n_splits + split) * 2 + t;
+        const bool direct = min(sp.n_tiles, p.n_splits) == 1;          // this CTA alone has the row's keys
+        const int64_t slot = ((static_cast<int64_t>(kvh) * p.n_pairs + pair) * p.n_splits + split) * NQ + (two ? t : 0);
         float* po = p.part_o + (slot * p.row_pitch + row) * HD;
+        const int grow = (2 * pair + (two ? t : 0)) * kBM + row;
+        uint16_t* out = p.out + (static_cast<int64_t>(node) * p.n_q + kvh * p.group + grow % p.group) * HD;
+        const float inv = l_sum == 0.f ? 0.f : 1.f / l_sum;
         const bool fix = *odd_flag != 0;
-#pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
+        const uint32_t t_other = tmem + 256 * (t ^ 1) + lane_off + kBN;
+        // columns of 32: this warp's share
+        const int c_lo = other && t == 1 ? HD / 64 : 0, c_hi = other && t == 0 ? HD / 64 : HD / 32;
+        for (int c = c_lo; c < c_hi; ++c) {
           uint32_t o[32];
           tmem_ld32(tO + c * 32, o);
-          tmem_wait_ld();
+          if (other) {
+            uint32_t y[32];
+            tmem_ld32(t_other + c * 32, y);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              o[e] = __float_as_uint(__uint_as_float(o[e]) * w_own + __uint_as_float(y[e]) * w_other);
+          } else {
+            tmem_wait_ld();
+          }
           if (row < n_rows && fix) {
-            // non-finite elements of the V rows this row sees in this slot's key tiles
-            for (int g = max(m0, two ? 0 : t); g < n; ++g) {
-              if (!two && ((g ^ t) & 1)) continue;
+            // non-finite elements of the V rows this row sees in this CTA's key tiles
+            for (int g = m0; g < n; ++g) {
               const int off = static_cast<int>(static_cast<int64_t>(j0 + g) * kBN - sp.n_ctx);
               for (int b = max(0, -off); b < kBN && off + b < p.n_nodes; ++b) {
                 const int j = off + b;
@@ -470,16 +506,20 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             }
           }
           if (row < n_rows) {
+            if (direct) {
+              store_chunk<DT>(out + c * 32, o, inv, false);
+            } else {
 #pragma unroll
-            for (int h = 0; h < 4; ++h)
-              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                           :: "l"(po + c * 32 + 8 * h), "r"(o[8 * h]), "r"(o[8 * h + 1]), "r"(o[8 * h + 2]),
-                              "r"(o[8 * h + 3]), "r"(o[8 * h + 4]), "r"(o[8 * h + 5]), "r"(o[8 * h + 6]),
-                              "r"(o[8 * h + 7]) : "memory");
+              for (int h = 0; h < 4; ++h)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                             :: "l"(po + c * 32 + 8 * h), "r"(o[8 * h]), "r"(o[8 * h + 1]), "r"(o[8 * h + 2]),
+                                "r"(o[8 * h + 3]), "r"(o[8 * h + 4]), "r"(o[8 * h + 5]), "r"(o[8 * h + 6]),
+                                "r"(o[8 * h + 7]) : "memory");
+            }
           }
           __syncwarp();
         }
-        if (row < n_rows) p.part_ml[slot * p.row_pitch + row] = make_float2(m_used, l_sum);
+        if (row < n_rows && !direct && (two || t == 0)) p.part_ml[slot * p.row_pitch + row] = make_float2(m_used, l_sum);
       }
     }
   }
@@ -497,44 +537,53 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 }
 
 // Merge of the splits, a warp per query row: O = sum_i w_i O_i / sum_i w_i l_i,
-// w_i = 2^(m_i - M) over the row's slots that hold a key tile, in their order.  A
-// row that sees nothing has every l_i = 0 and gets zeros.
+// w_i = 2^(m_i - M) over the splits that hold a key tile, in their order, eight O
+// loads in flight.  A row that sees nothing has every l_i = 0 and gets zeros.
+// (With one such split the attention kernel has written the output.)
 template <int DT, int HD>
 __global__ void __launch_bounds__(kTreeMergeWarps * 32)
 tree_merge_kernel(const TreeParams p, int n_kv) {
-  using E = Elem<DT>;
-  constexpr int kD = HD / 32;
-  __shared__ float s_w[kTreeMergeWarps][2 * kTreeMaxSplits];
+  constexpr int kD = HD / 32, kAhead = 8;
+  using Vec = typename std::conditional<kD == 4, float4, float2>::type;
+  __shared__ float s_w[kTreeMergeWarps][kTreeMaxSplits];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t gr = static_cast<int64_t>(blockIdx.x) * kTreeMergeWarps + warp;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (gr >= static_cast<int64_t>(n_kv) * p.rows) return;
-  const TreeSpan sp = tree_span(p);
-  if (!sp.ok) return;                                  // reported by the attention kernel
   const int kvh = static_cast<int>(gr / p.rows), row = static_cast<int>(gr % p.rows);
   const int qt = row / kBM, pair = qt / 2, r = row % kBM;
-  const bool two = (qt | 1) < p.n_qt;
-  // slot of index i: split i with the row's tile, or split i / 2 with half i & 1 of its key tiles
-  const int n_i = two ? p.n_splits : 2 * p.n_splits;
-  const int64_t slot0 = (static_cast<int64_t>(kvh) * p.n_pairs + pair) * p.n_splits * 2;
-  auto slot_of = [&](int i) { return two ? slot0 + 2 * i + (qt & 1) : slot0 + i; };
-  auto holds = [&](int i) {
-    const int s = two ? i : i >> 1;
-    return split_start(sp.n_tiles, p.n_splits, s + 1) - split_start(sp.n_tiles, p.n_splits, s) > (two ? 0 : (i & 1));
+  const int per = p.n_qt == 1 ? 1 : 2;                 // slots of a split
+  const int64_t slot0 = (static_cast<int64_t>(kvh) * p.n_pairs + pair) * p.n_splits * per +
+                        ((qt | 1) < p.n_qt ? qt & 1 : 0);
+  const float2* ml = p.part_ml + slot0 * p.row_pitch + r;
+  const float* po = p.part_o + (slot0 * p.row_pitch + r) * HD + lane * kD;
+  const int64_t step = static_cast<int64_t>(per) * p.row_pitch;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const TreeSpan sp = tree_span(p);
+  if (!sp.ok) return;                                  // reported by the attention kernel
+  const int n = min(sp.n_tiles, p.n_splits);           // splits 0 .. n - 1 hold key tiles
+  if (n == 1) return;
+  Vec x[kAhead];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (i0 + k < n) x[k] = *reinterpret_cast<const Vec*>(po + (i0 + k) * step * HD);
   };
+  load(0);                                             // on its way beside the (m, l) pairs
+  float2 mine[kTreeMaxSplits / 32];
   float M = -INFINITY;
-  for (int i = lane; i < n_i; i += 32) {
-    const float2 ml = holds(i) ? p.part_ml[slot_of(i) * p.row_pitch + r] : make_float2(-INFINITY, 0.f);
-    if (ml.y != 0.f) M = fmaxf(M, ml.x);
+#pragma unroll
+  for (int q = 0; q < kTreeMaxSplits / 32; ++q) {
+    mine[q] = lane + 32 * q < n ? ml[(lane + 32 * q) * step] : make_float2(-INFINITY, 0.f);
+    if (mine[q].y != 0.f) M = fmaxf(M, mine[q].x);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   float lsum = 0.f;
-  for (int i = lane; i < n_i; i += 32) {
-    const float2 ml = holds(i) ? p.part_ml[slot_of(i) * p.row_pitch + r] : make_float2(-INFINITY, 0.f);
-    const float w = ml.y != 0.f ? ex2(ml.x - M) : 0.f;
-    s_w[warp][i] = holds(i) ? w : -1.f;
-    lsum += ml.y != 0.f ? w * ml.y : 0.f;
+#pragma unroll
+  for (int q = 0; q < kTreeMaxSplits / 32; ++q) {
+    const float w = mine[q].y != 0.f ? ex2(mine[q].x - M) : 0.f;
+    s_w[warp][lane + 32 * q] = w;
+    lsum += mine[q].y != 0.f ? w * mine[q].y : 0.f;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
@@ -542,21 +591,18 @@ tree_merge_kernel(const TreeParams p, int n_kv) {
   float acc[kD];
 #pragma unroll
   for (int d = 0; d < kD; ++d) acc[d] = 0.f;
-#pragma unroll 8
-  for (int i = 0; i < n_i; ++i) {
-    const float w = s_w[warp][i];
-    if (w < 0.f) continue;                             // nothing was written there
-    const float* po = p.part_o + (slot_of(i) * p.row_pitch + r) * HD + lane * kD;
-    if constexpr (kD == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(po);
-      acc[0] = fmaf(w, x.x, acc[0]);
-      acc[1] = fmaf(w, x.y, acc[1]);
-      acc[2] = fmaf(w, x.z, acc[2]);
-      acc[3] = fmaf(w, x.w, acc[3]);
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(po);
-      acc[0] = fmaf(w, x.x, acc[0]);
-      acc[1] = fmaf(w, x.y, acc[1]);
+  for (int i0 = 0; i0 < n; i0 += kAhead) {
+    if (i0 > 0) load(i0);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (i0 + k >= n) break;
+      const float w = s_w[warp][i0 + k];
+      acc[0] = fmaf(w, x[k].x, acc[0]);
+      acc[1] = fmaf(w, x[k].y, acc[1]);
+      if constexpr (kD == 4) {
+        acc[2] = fmaf(w, x[k].z, acc[2]);
+        acc[3] = fmaf(w, x[k].w, acc[3]);
+      }
     }
   }
   const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
@@ -582,7 +628,7 @@ static TreeLayout tree_layout(int n_nodes, int64_t cap, int n_q_heads, int n_kv_
   const int64_t sms = std::min(attn_sm_count(), kTreeMaxSplits);
   t.n_splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / units, (cap + kBN - 1) / kBN)));
   t.row_pitch = (std::min(t.rows, kBM) + 7) / 8 * 8;
-  const size_t slots = static_cast<size_t>(units) * t.n_splits * 2;
+  const size_t slots = static_cast<size_t>(units) * t.n_splits * (t.n_qt == 1 ? 1 : 2);
   t.off_o = (slots * t.row_pitch * sizeof(float2) + 255) & ~static_cast<size_t>(255);
   t.bytes = t.off_o + slots * t.row_pitch * head_dim * sizeof(float);
   return t;
