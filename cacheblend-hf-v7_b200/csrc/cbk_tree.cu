@@ -194,16 +194,24 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   } else if (warp >= 4) {
     // Q tiles in the layout a 128-byte-swizzled TMA copy leaves: 16-byte piece c of
     // row r at piece c ^ (r & 7); rows that do not exist are zero
-    constexpr int kVec = HD / 8;
-    const int n_q_tiles = two ? 2 : 1;
-    for (int i = threadIdx.x - 128; i < n_q_tiles * kBM * kVec; i += kTreeThreads - 128) {
-      const int r = i / kVec, c = i % kVec;
-      const int row = 2 * pair * kBM + r;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (row < p.rows)
-        x = ld_vec(p.q + (static_cast<int64_t>(row / p.group) * p.n_q + kvh * p.group + row % p.group) * HD + c * 8);
-      *reinterpret_cast<uint4*>(sbase + (r / kBM) * L::kQBytes + (c >> 3) * (kBM * 128) + (r % kBM) * 128 +
-                                ((c ^ r) & 7) * 16) = x;
+    constexpr int kVec = HD / 8, kStep = (kTreeThreads - 128) / kVec, kAhead = kBM / kStep;
+    const int c = threadIdx.x % kVec, r0 = (threadIdx.x - 128) / kVec;
+    const int row0 = 2 * pair * kBM;
+    for (int r = r0; r < (two ? 2 : 1) * kBM; r += kStep * kAhead) {
+      uint4 x[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int row = row0 + r + k * kStep, node = row / p.group;
+        x[k] = make_uint4(0, 0, 0, 0);
+        if (row < p.rows)
+          x[k] = ld_vec(p.q + (static_cast<int64_t>(node) * p.n_q + kvh * p.group + row - node * p.group) * HD + c * 8);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int at = r + k * kStep;
+        *reinterpret_cast<uint4*>(sbase + (at / kBM) * L::kQBytes + (c >> 3) * (kBM * 128) + (at % kBM) * 128 +
+                                  ((c ^ at) & 7) * 16) = x[k];
+      }
     }
     fence_proxy_async_smem();
   }
@@ -557,8 +565,9 @@ tree_merge_kernel(const TreeParams p, int n_kv) {
   const float2* ml = p.part_ml + slot0 * p.row_pitch + r;
   const float* po = p.part_o + (slot0 * p.row_pitch + r) * HD + lane * kD;
   const int64_t step = static_cast<int64_t>(per) * p.row_pitch;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // (n_ctx is no result of the attention kernel: whoever writes it is done)
   const TreeSpan sp = tree_span(p);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!sp.ok) return;                                  // reported by the attention kernel
   const int n = min(sp.n_tiles, p.n_splits);           // splits 0 .. n - 1 hold key tiles
   if (n == 1) return;
