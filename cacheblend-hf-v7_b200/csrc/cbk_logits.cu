@@ -26,9 +26,6 @@
 // logits (16 or 32 bytes), kLgBatch loads in flight, the first batch before the
 // counting starts.  Rows that do not lie on 16-byte boundaries are read element by
 // element, neighbouring lanes on neighbouring elements.
-#ifndef LG_REMOTE
-#define LG_REMOTE 0
-#endif
 #include <algorithm>
 
 #include "cbk_common.cuh"
@@ -135,9 +132,6 @@ process_logits_kernel(const LogitsParams p) {
   __shared__ unsigned long long s_row[kLgCluster];       // rank 0: one key per CTA of the cluster
   const int rank = static_cast<int>(cluster_rank()), tid = threadIdx.x;
   const int n_clusters = gridDim.x / kLgCluster;
-#if LG_REMOTE
-  const uint32_t base = smem_u32(s_count);
-#endif
   // the CTA's share of the vocabulary: every kLgCluster-th block of kLgBlock tokens,
   // one after the other at offsets [0, seg) of its counts
   auto token_at = [&](int o) { return ((o / kLgBlock) * kLgCluster + rank) * kLgBlock + o % kLgBlock; };
@@ -148,25 +142,12 @@ process_logits_kernel(const LogitsParams p) {
     }
     const uint32_t block = static_cast<uint32_t>(t) / kLgBlock;
     const uint32_t o = (block / kLgCluster) * kLgBlock + static_cast<uint32_t>(t) % kLgBlock;
-#if LG_REMOTE
-    const uint32_t a = map_rank(base + 4u * o, block % kLgCluster);
-    if (made) asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(a), "r"(by) : "memory");
-    else asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(a), "r"(kLgPrompt) : "memory");
-#else
     if (block % kLgCluster != rank) return;
     if (made) atomicAdd(s_count + o, by);
     else atomicOr(s_count + o, kLgPrompt);
-#endif
   };
-#if LG_REMOTE
-  constexpr int kStep = kLgCluster * kLgThreads;
-  const int first = rank * kLgThreads + tid;
-#else
-  constexpr int kStep = kLgThreads;
-  const int first = tid;
-#endif
   auto add_path = [&](int row, uint32_t by) {
-    for (int j = first; j < p.n_tree; j += kStep)
+    for (int j = tid; j < p.n_tree; j += kLgThreads)
       if ((p.tree_words[row * p.tree_stride + j / 32] >> (j % 32)) & 1u) add(p.tree_tokens[j], true, by);
   };
 
@@ -197,13 +178,13 @@ process_logits_kernel(const LogitsParams p) {
           }
           const int64_t* h = p.history + row * p.hist_stride;
           constexpr int kAhead = 8;
-          for (int64_t i = first; i < len; i += kAhead * kStep) {
+          for (int64_t i = tid; i < len; i += kAhead * kLgThreads) {
             int64_t t[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) t[k] = i + k * kStep < len ? __ldg(h + i + k * kStep) : 0;
+            for (int k = 0; k < kAhead; ++k) t[k] = i + k * kLgThreads < len ? __ldg(h + i + k * kLgThreads) : 0;
 #pragma unroll
             for (int k = 0; k < kAhead; ++k)
-              if (i + k * kStep < len) add(t[k], i + k * kStep >= prompt, 1u);
+              if (i + k * kLgThreads < len) add(t[k], i + k * kLgThreads >= prompt, 1u);
           }
         }
         add_path(row, 1u);
