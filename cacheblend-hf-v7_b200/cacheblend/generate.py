@@ -10,30 +10,85 @@ into cache row p (``rope_scatter`` with one index), and attention of the one
 query row over rows [0, p] (``decode_attn``: split over the keys, HBM-bound).  Token 1 is the argmax of
 the last prefill row, as in the reference; decoding stops after
 ``max_new_tokens`` tokens or at ``eos_token_id``.
+
+Both decoders (this one and ``generate_drafted``) can penalise repeated tokens,
+add a bias and restrict the vocabulary; ``process_logits`` then changes each
+row and chooses its token on the device.
 """
 from __future__ import annotations
 
 import torch
 
 from cacheblend import ops
-from cacheblend.chunker import Chunk
+from cacheblend.chunker import Chunk, fused_input_ids
 from cacheblend.fusor import _MLPS, _SILUS, _fused_w, _mlp, _norm, _qkv, _selective_prefill, fuse_selective
 from cacheblend.kv_store import KVStore
+
+
+class _Choice:
+    """How a decode chooses tokens: penalties over the prompt's and the made
+    tokens, bias and allowed tokens (``process_logits``), or plain argmax when
+    none is asked for.  Holds the token history on the device: ``history[:length]``
+    are the tokens so far, the first ``n_prompt`` of them the prompt's."""
+
+    def __init__(self, device, vocab: int, chunks: list[Chunk], spare: int, repetition_penalty: float,
+                 presence_penalty: float, frequency_penalty: float, logit_bias: torch.Tensor | None,
+                 allowed_tokens: torch.Tensor | None, status: torch.Tensor | None):
+        self.penalties = dict(repetition=float(repetition_penalty), presence=float(presence_penalty),
+                              frequency=float(frequency_penalty))
+        if not repetition_penalty > 0:
+            raise ValueError(f"repetition_penalty must be > 0, got {repetition_penalty}")
+        self.counted = (repetition_penalty, presence_penalty, frequency_penalty) != (1.0, 0.0, 0.0)
+        self.status = status
+        self.bias = self.mask = None
+        if logit_bias is not None:
+            if logit_bias.numel() != vocab:
+                raise ValueError(f"logit_bias must have {vocab} entries, got {logit_bias.numel()}")
+            self.bias = logit_bias.reshape(-1).to(device=device, dtype=torch.float32)
+        if allowed_tokens is not None:
+            if allowed_tokens.dtype != torch.bool or allowed_tokens.numel() != vocab:
+                raise ValueError(f"allowed_tokens must be bool with {vocab} entries, got "
+                                 f"{allowed_tokens.dtype}{list(allowed_tokens.shape)}")
+            self.mask = ops.mask_words(allowed_tokens).to(device)
+        self.plain = not self.counted and self.bias is None and self.mask is None
+        if self.counted:
+            ids = fused_input_ids(chunks, device=device).reshape(-1)
+            self.history = torch.zeros((ids.numel() + spare,), dtype=torch.int64, device=device)
+            self.history[:ids.numel()].copy_(ids)
+            self.length = torch.full((1,), ids.numel(), dtype=torch.int64, device=device)
+            self.n_prompt = self.length.clone()
+
+    def __call__(self, rows: torch.Tensor, return_rows: bool = False, **tree):
+        """(rows as they chose or None, tokens) of logits rows [n][vocab]; with
+        ``tree_tokens`` / ``tree_words`` of the nodes of a drafted tree."""
+        if self.plain:
+            return (rows if return_rows else None), rows.argmax(-1)
+        past = dict(history=self.history, lengths=self.length, n_prompt=self.n_prompt, **tree) if self.counted else {}
+        return ops.process_logits(rows, **past, **self.penalties, bias=self.bias, mask_words=self.mask,
+                                  return_logits=return_rows, status=self.status)
+
+    def made(self, token: torch.Tensor) -> None:
+        """Append one chosen token to the history (on the device)."""
+        if self.counted:
+            self.history.index_copy_(0, self.length, token.view(1))
+            self.length.add_(1)
 
 
 class _DecodeState:
     """Static device buffers of a decode: the current token and position, the
     attention workspace, and the chosen tokens / logits rows by step."""
 
-    def __init__(self, lw, pre, n_new: int, first_row: torch.Tensor, keep_rows: bool):
+    def __init__(self, lw, pre, n_new: int, first_row: torch.Tensor, keep_rows: bool, choice: _Choice):
         device, geo = lw.device, pre.geo
         cap = pre.fused_k.shape[1]
         self.tokens = torch.zeros((n_new,), dtype=torch.int64, device=device)
         self.rows = torch.zeros((n_new, first_row.shape[-1]), dtype=first_row.dtype, device=device) if keep_rows else None
-        first = first_row.argmax().view(1)
+        self.choice = choice
+        row, first = choice(first_row.view(1, -1), keep_rows)
         self.tokens[0:1].copy_(first)
+        choice.made(first)
         if keep_rows:
-            self.rows[0].copy_(first_row)
+            self.rows[0].copy_(row[0])
         self.token = first.view(1, 1).clone()
         self.pos = torch.full((1,), pre.S, dtype=torch.int64, device=device)
         self.base = pre.S - 1               # token t of the output was chosen at position base + t
@@ -106,7 +161,8 @@ def _decode_step(lw, pre, st: _DecodeState, status):
         o = _lin1(attn.o_proj, a.unsqueeze(0))
         m = _mlp1(layer, _norm(layer.post_attention_layernorm, h, delta=o, sum_out=h, status=status), w_gu)
     row = _lin1(lw.model.lm_head, _norm(inner.norm, h, delta=m, status=status))[0, -1]
-    nxt = row.argmax().view(1)
+    row, nxt = st.choice(row.view(1, -1), st.rows is not None)
+    st.choice.made(nxt)
     slot = st.pos - st.base
     st.tokens.index_copy_(0, slot, nxt)
     if st.rows is not None:
@@ -118,7 +174,9 @@ def _decode_step(lw, pre, st: _DecodeState, status):
 def generate_greedy(layerwise_model, chunks: list[Chunk], kv_store: KVStore, max_new_tokens: int,
                     recompute_ratio: float = 0.15, check_layer: int = 1, eos_token_id: int | None = None,
                     rope_mode: str = "ref", status: torch.Tensor | None = None, return_logits: bool = False,
-                    use_graph: bool = True):
+                    use_graph: bool = True, repetition_penalty: float = 1.0, presence_penalty: float = 0.0,
+                    frequency_penalty: float = 0.0, logit_bias: torch.Tensor | None = None,
+                    allowed_tokens: torch.Tensor | None = None):
     """CacheBlend selective prefill, then greedy decode over the blended cache.
 
     Returns the generated token ids (token 1 from the prefill's last row), and
@@ -128,19 +186,33 @@ def generate_greedy(layerwise_model, chunks: list[Chunk], kv_store: KVStore, max
     after the first ``eos_token_id``, so a run that meets EOS early decodes the
     remaining steps for nothing but returns what the reference returns.  The
     shortcut cases of fuse_selective (ratio 0, ratio >= 1, one chunk) run the
-    reference path: HF prefill and HF decode with ``past_key_values``."""
+    reference path: HF prefill and HF decode with ``past_key_values``.
+
+    ``repetition_penalty`` divides the positive and multiplies the negative logits
+    of tokens that the prompt or the output has; ``frequency_penalty`` (per
+    occurrence) and ``presence_penalty`` are taken off those that the output has.
+    Then ``logit_bias`` (fp32, one per vocabulary entry) is added, and tokens
+    outside ``allowed_tokens`` (bool, one per entry) are excluded.  The returned
+    rows are those that chose, with all of this done."""
     if max_new_tokens <= 0:
         return ([], []) if return_logits else []
     lw = layerwise_model
     selective = 0 < recompute_ratio < 1 and len(chunks) > 1
     tokens, rows = [], []
     with torch.inference_mode():
+        choice = _Choice(lw.device, lw.model.config.vocab_size, chunks, max_new_tokens, repetition_penalty,
+                         presence_penalty, frequency_penalty, logit_bias, allowed_tokens, status)
         if not selective:
             out = fuse_selective(lw, chunks, kv_store, recompute_ratio, check_layer, return_layerwise_output=True)
             row = out.logits[0, -1]
             cache = out.past_key_values
             for i in range(max_new_tokens):
-                nxt = row.argmax()
+                if choice.plain:
+                    nxt = row.argmax()
+                else:
+                    row, nxt = choice(row.view(1, -1), True)
+                    row = row[0]
+                    choice.made(nxt)
                 tokens.append(int(nxt.item()))
                 rows.append(row)
                 if (eos_token_id is not None and tokens[-1] == eos_token_id) or i + 1 == max_new_tokens:
@@ -151,7 +223,7 @@ def generate_greedy(layerwise_model, chunks: list[Chunk], kv_store: KVStore, max
             # only the last prefill row is read: lm_head on that row alone
             pre = _selective_prefill(lw, chunks, kv_store, recompute_ratio, check_layer, rope_mode, status,
                                      None, extra_tokens=max_new_tokens, logits_rows="last")
-            st = _DecodeState(lw, pre, max_new_tokens, pre.logits[0, -1], return_logits)
+            st = _DecodeState(lw, pre, max_new_tokens, pre.logits[0, -1], return_logits, choice)
             n_steps = max_new_tokens - 1
             if n_steps >= 1:
                 _decode_step(lw, pre, st, status)          # eager: first use sets up every kernel

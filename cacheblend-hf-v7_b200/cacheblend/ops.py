@@ -704,6 +704,18 @@ def tree_words(parents: Sequence[int], width: int | None = None) -> tuple[torch.
     return torch.from_numpy(words), torch.from_numpy(depth)
 
 
+def mask_words(allowed: torch.Tensor) -> torch.Tensor:
+    """int32 bit words (..., ceil(n / 32)) of a bool tensor (..., n), on its device:
+    bit t % 32 of word t / 32 is entry t (process_logits' ``mask_words``)."""
+    if allowed.dtype != torch.bool:
+        raise ValueError(f"mask_words: bool tensor expected, got {allowed.dtype}")
+    n = allowed.shape[-1]
+    wide = torch.zeros((*allowed.shape[:-1], (n + 31) // 32 * 32), dtype=torch.int64, device=allowed.device)
+    wide[..., :n] = allowed
+    words = (wide.view(*allowed.shape[:-1], -1, 32) << torch.arange(32, device=allowed.device)).sum(-1)
+    return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+
+
 def _word_rows(words: torch.Tensor) -> tuple[torch.Tensor, int]:
     """2-D bit words and their row stride; broadcast or overlapping rows are copied apart."""
     if words.shape[0] <= 1:

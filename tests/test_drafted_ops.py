@@ -124,3 +124,42 @@ def test_reference_bounds_catch_mistakes():
     assert ((more - out).abs() > b)[0].any() and ((more - out).abs() <= b)[1:].all()
     row, tok = ref.logits(torch.tensor([[1.0, 3.0, 2.9, -1.0]]), history=torch.tensor([1, 3]), repetition=1.5)
     assert np.allclose(row.numpy(), [[1.0, 2.0, 2.9, -1.5]]) and tok.tolist() == [2]
+
+
+def test_mask_words():
+    from cacheblend import ops
+    a = torch.zeros((2, 70), dtype=torch.bool)
+    a[0, [0, 31, 32, 69]] = True
+    a[1] = True
+    w = ops.mask_words(a)
+    assert w.dtype == torch.int32 and w.tolist() == [[1 - (1 << 31), 1, 32], [-1, -1, 63]]
+    assert ops.mask_words(a[1]).tolist() == [-1, -1, 63]
+    with pytest.raises(ValueError):
+        ops.mask_words(a.int())
+
+
+def test_prompt_lookup_tree():
+    from cacheblend import prompt_lookup_tree as look
+    #      0  1  2  3  4  5  6  7  8  9
+    ids = [5, 6, 7, 8, 9, 6, 7, 1, 6, 7]
+    # the tail (6, 7) is followed by 1, 6, 7 (latest first), then by 8, 9, 6, 7, 1, 6, 7
+    tokens, parents = look(ids, 20)
+    assert tokens == [1, 6, 7, 8, 9, 6, 7, 1, 6, 7] and parents == [-1, 0, 1, -1, 3, 4, 5, 6, 7, 8]
+    assert look(ids, 4) == ([1, 6, 7, 8], [-1, 0, 1, -1])
+    assert look(ids, 5, depth=2) == ([1, 6, 8, 9], [-1, 0, -1, 2])
+    assert look(ids, 0) == ([], [])
+    # alike beginnings share their nodes
+    assert look([1, 2, 3, 4, 1, 2, 3, 5, 1], 9, depth=3) == ([2, 3, 5, 4], [-1, 0, 1, 1])
+    # nothing repeats; one token; none
+    assert look([1, 2, 3], 5) == ([], []) and look([4], 5) == ([], []) and look([], 5) == ([], [])
+    assert look([3, 3], 5) == ([3], [-1])
+
+
+def test_accepted_path():
+    from cacheblend.drafted import _accept
+    tokens, parents = [9, 4, 5, 6, 7, 5], [-1, 0, 0, 1, 3, 1]
+    assert _accept(tokens, parents, [1, 0, 0, 0, 0, 0]) == [0]
+    assert _accept(tokens, parents, [4, 6, 0, 7, 2, 0]) == [0, 1, 3, 4]
+    assert _accept(tokens, parents, [4, 5, 0, 7, 2, 0]) == [0, 1, 5]
+    assert _accept(tokens, parents, [5, 5, 0, 0, 0, 0]) == [0, 2]
+    assert _accept([9], [-1], [3]) == [0]
