@@ -58,6 +58,7 @@ SIGNATURES = {
     "cbk_norm_rope_scatter": (_i32, [ctypes.c_char_p, _vp]),
     "cbk_tree_attn_workspace_bytes": (_sz, [_i32, _i64, _i32, _i32, _i32]),
     "cbk_tree_attn": (_i32, [ctypes.c_char_p, _vp]),
+    "cbk_process_logits_workspace_bytes": (_sz, [_i64, _i64]),
     "cbk_process_logits": (_i32, [ctypes.c_char_p, _vp]),
 }
 
@@ -66,7 +67,7 @@ SIGNATURES = {
 PACK = {
     "cbk_norm_rope_scatter": struct.Struct("=20q7if"),
     "cbk_tree_attn": struct.Struct("=13q5if"),
-    "cbk_process_logits": struct.Struct("=23q3i3f"),
+    "cbk_process_logits": struct.Struct("=25q3i3f"),
 }
 
 

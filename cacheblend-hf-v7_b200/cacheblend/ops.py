@@ -519,7 +519,7 @@ def _launcher(name: str, n_launches: int):
 
 _norm_rope_scatter = _launcher("norm_rope_scatter", 1)
 _tree_attn = _launcher("tree_attn", 2)
-_process_logits = _launcher("process_logits", 1)
+_process_logits = _launcher("process_logits", 2)
 
 
 def _same_device(first: torch.Tensor, *others) -> torch.device:
@@ -833,10 +833,16 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, le
         raise ValueError("process_logits: repetition must be > 0 and no penalty NaN")
     if repetition == 1.0 and presence == 0.0 and frequency == 0.0:
         hist_cap = n_tree = 0                    # nothing depends on the counts
+    ws = ws_bytes = 0
+    if hist_cap and rows > 1 and not (hist_stride or len_stride or prompt_stride):
+        ws_bytes = N.LIB.cbk_process_logits_workspace_bytes(rows, vocab)
+        if ws_bytes:
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            ws = workspace.data_ptr()
     if rows == 1:                                # one row's stride says nothing
         row_stride = out_stride = vocab
     _process_logits(dev, logits.data_ptr(), hist, lens, prompt, bias_p, mask_p, toks, words, out_p, tokens.data_ptr(),
-                    0 if status is None else status.data_ptr(), row_stride, rows, vocab, hist_stride, hist_cap,
-                    len_stride, prompt_stride, bias_stride, mask_stride, tree_stride, out_stride, n_tree, code,
-                    out_code, repetition, presence, frequency)
+                    0 if status is None else status.data_ptr(), ws, row_stride, rows, vocab, hist_stride, hist_cap,
+                    len_stride, prompt_stride, bias_stride, mask_stride, tree_stride, out_stride, ws_bytes, n_tree,
+                    code, out_code, repetition, presence, frequency)
     return out, tokens

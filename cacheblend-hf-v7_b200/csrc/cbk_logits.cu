@@ -12,20 +12,20 @@
 // is the first largest x, NaN counting as larger than any number; a row whose
 // mask allows nothing is all -inf and chooses token 0.
 //
-// A cluster of CTAs takes a row (several rows, one after the other, when there are
-// more rows than clusters fit), each CTA a contiguous segment of the vocabulary,
-// whose counts it keeps in its shared memory (bits 0-30 made, bit 31 in the
-// prompt).  The history is read once per row -- once per cluster when the rows
-// share it -- the CTAs sharing its positions and adding to the owner's counts
-// through distributed shared memory; a tree node's path is added for its row and
-// taken back after it.  The row's choice is a maximum over 64-bit keys (order of x,
-// then lowest index) in the CTA and over the cluster: one launch, no workspace, no
-// order of atomics that could show.
+// process_logits_kernel: a cluster of CTAs takes a row (several rows, one after the
+// other, when there are more rows than clusters fit), each CTA every n-th block of
+// 128 tokens of the vocabulary.  A thread takes vectors of 8 logits (16 or 32 bytes),
+// kBatch loads in flight, the first batch before any counting.  The row's choice is a
+// maximum over 64-bit keys (order of x, then lowest index) in the CTA and over the
+// cluster, so no order of atomics shows.  Rows that do not lie on 16-byte boundaries
+// are read element by element, neighbouring lanes on neighbouring elements.
 //
-// Bound by memory for many rows, by latency for few: a thread takes vectors of 8
-// logits (16 or 32 bytes), kLgBatch loads in flight, the first batch before the
-// counting starts.  Rows that do not lie on 16-byte boundaries are read element by
-// element, neighbouring lanes on neighbouring elements.
+// Counts per token (bits 0-30 made, bit 31 in the prompt) come about in one of two
+// ways.  Few rows, or a history per row: a CTA reads the whole history and counts what
+// falls into its share, in its shared memory, with no second launch.  Many rows of one
+// history: every cluster would do that again, so count_tokens_kernel does it once, in
+// the workspace, and the rows read the counts from L2.  What a drafted tree's node
+// adds is a short list per row; a bit per vector of 8 tokens says where to look it up.
 #include <algorithm>
 
 #include "cbk_common.cuh"
@@ -35,11 +35,15 @@ namespace cbk {
 int ensure_smem_attr(const void* func, int bytes);   // cbk_api.cu
 
 constexpr int kLgThreads = 512;
-constexpr int kLgCluster = 8;
-constexpr int kLgBatch = 4;
 constexpr int kLgBlock = 128;                           // tokens of a CTA's blocks
-constexpr int kLgMaxClusters = 36;                      // two CTAs on each of 148 SMs, whole clusters
-constexpr int kLgMaxVocab = kLgCluster * 56 * 1024;   // a segment's counts fit in shared memory
+constexpr int kLgMaxVocab = 458752;
+constexpr int kLgMaxTree = 1024;
+constexpr int kLgMaxSmem = 224 * 1024;
+constexpr int kLgCountCtas = 8;                         // CTAs that count a shared history
+// Rows from which a shared history is counted once (64 rows of 128256 after 24 K
+// tokens: 29.6 us against 52.9 with every cluster counting; 16 rows after 5 K: 14.5
+// against 14.1), and clusters that fit side by side, two CTAs to an SM.
+constexpr int kLgManyRows = 24, kLgFit8 = 30, kLgFit4 = 66;
 constexpr uint32_t kLgPrompt = 0x80000000u;
 
 struct LogitsParams {
@@ -48,12 +52,13 @@ struct LogitsParams {
   const int64_t *history, *lengths, *n_prompt, *tree_tokens;
   const uint32_t *mask, *tree_words;
   const float* bias;
+  uint32_t* counts;               // a shared history's counts in the workspace, or null
   int64_t* tokens;
   int32_t* status;
   int64_t row_stride, out_stride, hist_stride, hist_cap, len_stride, prompt_stride, bias_stride, mask_stride,
       tree_stride;
-  int rows, vocab, seg, n_tree, counted, shared;
-  float repetition, presence, frequency;
+  int rows, vocab, seg, n_tree, shared, log_cluster;
+  float repetition, inv_repetition, presence, frequency;
 };
 
 // order of fp32 values as unsigned integers: -inf < ... < -0 = +0 < ... < inf < NaN
@@ -86,6 +91,16 @@ template <int DT>
 __device__ __forceinline__ void store1(void* p, int64_t i, float x) {
   if constexpr (DT == CBK_F32) static_cast<float*>(p)[i] = x;
   else static_cast<uint16_t*>(p)[i] = Elem<DT>::from_f(x);
+}
+
+// x / b for x > 0, correctly rounded, from y = the rounded 1 / b: with q = RN(x y), the
+// remainder r = x - q b is exact in one FMA, and RN(q + r y) is the rounded quotient
+// (Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990) as long as nothing under- or overflows on the way.
+__device__ __forceinline__ float divide(float x, float b, float y) {
+  if (!(x > 1e-20f && x < 1e20f)) return __fdiv_rn(x, b);
+  const float q = __fmul_rn(x, y);
+  return __fmaf_rn(__fmaf_rn(-q, b, x), y, q);
 }
 
 // max that propagates NaN
@@ -123,35 +138,86 @@ struct Raw {
   }
 };
 
+// One cluster: clear the counts, then add the tokens of the history that all rows share.
+__global__ void __launch_bounds__(1024)
+count_tokens_kernel(const LogitsParams p) {
+  const int rank = static_cast<int>(cluster_rank());
+  const int tid = rank * 1024 + threadIdx.x;
+  constexpr int kStep = kLgCountCtas * 1024;
+  uint32_t* counts = p.counts;
+  const int cells = (p.vocab + 127) / 128 * 128;
+  for (int i = tid; i < cells / 4; i += kStep)
+    reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
+  int64_t len = p.lengths ? *p.lengths : p.hist_cap;
+  const int64_t prompt = p.n_prompt ? *p.n_prompt : 0;
+  if (len < 0 || len > p.hist_cap) {
+    if (tid == 0) report(p.status, CBK_STATUS_BAD_INDEX);
+    len = len < 0 ? 0 : p.hist_cap;
+  }
+  const int64_t* h = p.history;
+  constexpr int kAhead = 4;
+  bool cleared = false, bad = false;
+  for (int64_t i0 = 0; i0 < len; i0 += kAhead * kStep) {
+    int64_t t[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (i0 + k * kStep + tid < len) t[k] = __ldg(h + i0 + k * kStep + tid);
+    if (!cleared) cluster_sync_all();                 // every count is zero before any is added to
+    cleared = true;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t i = i0 + k * kStep + tid;
+      if (i >= len) break;
+      if (t[k] < 0 || t[k] >= p.vocab) bad = true;
+      else if (i >= prompt) atomicAdd(counts + t[k], 1u);
+      else atomicOr(counts + t[k], kLgPrompt);
+    }
+  }
+  if (bad) report(p.status, CBK_STATUS_BAD_INDEX);
+  asm volatile("griddepcontrol.launch_dependents;");
+}
+
 template <int IN, int OUT, int VEC>
 __global__ void __launch_bounds__(kLgThreads, 2)
 process_logits_kernel(const LogitsParams p) {
-  constexpr int kBatch = VEC == 1 ? 8 : IN == CBK_F32 ? kLgBatch / 2 : kLgBatch;
-  extern __shared__ __align__(16) uint32_t s_count[];    // [seg] when the rows have a history
+  constexpr int kBatch = VEC == 1 ? 8 : IN == CBK_F32 ? 2 : 4;
+  // counts [seg] (when the CTA counts), path bits [seg / 256] and path [n_tree] (with a tree)
+  extern __shared__ __align__(16) uint32_t s_dyn[];
+  __shared__ int s_n_path;
   __shared__ unsigned long long s_best[kLgThreads / 32];
-  __shared__ unsigned long long s_row[kLgCluster];       // rank 0: one key per CTA of the cluster
+  __shared__ unsigned long long s_row[16];               // rank 0: one key per CTA of the cluster
   const int rank = static_cast<int>(cluster_rank()), tid = threadIdx.x;
-  const int n_clusters = gridDim.x / kLgCluster;
-  // the CTA's share of the vocabulary: every kLgCluster-th block of kLgBlock tokens,
-  // one after the other at offsets [0, seg) of its counts
-  auto token_at = [&](int o) { return ((o / kLgBlock) * kLgCluster + rank) * kLgBlock + o % kLgBlock; };
-  auto add = [&](int64_t t, bool made, uint32_t by) {
-    if (t < 0 || t >= p.vocab) {
-      if (rank == 0) report(p.status, CBK_STATUS_BAD_INDEX);
-      return;
-    }
-    const uint32_t block = static_cast<uint32_t>(t) / kLgBlock;
-    const uint32_t o = (block / kLgCluster) * kLgBlock + static_cast<uint32_t>(t) % kLgBlock;
-    if (block % kLgCluster != rank) return;
-    if (made) atomicAdd(s_count + o, by);
-    else atomicOr(s_count + o, kLgPrompt);
-  };
-  auto add_path = [&](int row, uint32_t by) {
-    for (int j = tid; j < p.n_tree; j += kLgThreads)
-      if ((p.tree_words[row * p.tree_stride + j / 32] >> (j % 32)) & 1u) add(p.tree_tokens[j], true, by);
-  };
+  const int n_clusters = gridDim.x >> p.log_cluster, cluster_mask = (1 << p.log_cluster) - 1;
+  const bool counts_here = p.history != nullptr && p.counts == nullptr;
+  uint32_t* s_count = s_dyn;
+  uint32_t* s_over = s_dyn + (counts_here ? p.seg : 0);
+  uint32_t* s_path = s_over + (p.n_tree > 0 ? (p.seg + 255) / 256 : 0);
 
-  for (int row = blockIdx.x / kLgCluster, turn = 0; row < p.rows; row += n_clusters, ++turn) {
+  // the CTA's share of the vocabulary: every n-th block of kLgBlock tokens, one after
+  // the other at offsets [0, seg)
+  auto token_at = [&](int o) { return (((o / kLgBlock) << p.log_cluster) + rank) * kLgBlock + o % kLgBlock; };
+  auto offset_of = [&](uint32_t t) {
+    return static_cast<int>(((t / kLgBlock) >> p.log_cluster) * kLgBlock + t % kLgBlock);
+  };
+  // (the low word alone says whose token it is; one outside the vocabulary is reported by one CTA)
+  auto ours = [&](int64_t t) { return (static_cast<int>(static_cast<uint32_t>(t) / kLgBlock) & cluster_mask) == rank; };
+  auto known = [&](int64_t t) {
+    if (static_cast<uint64_t>(t) < static_cast<uint64_t>(p.vocab)) return true;
+    report(p.status, CBK_STATUS_BAD_INDEX);
+    return false;
+  };
+  auto add = [&](int64_t t, bool made) {
+    if (!known(t)) return;
+    if (made) atomicAdd(s_count + offset_of(static_cast<uint32_t>(t)), 1u);
+    else atomicOr(s_count + offset_of(static_cast<uint32_t>(t)), kLgPrompt);
+  };
+  if (p.n_tree > 0) {
+    for (int i = tid; i < (p.seg + 255) / 256; i += kLgThreads) s_over[i] = 0;
+    if (tid == 0) s_n_path = 0;
+    __syncthreads();
+  }
+
+  for (int row = blockIdx.x >> p.log_cluster, turn = 0; row < p.rows; row += n_clusters, ++turn) {
     const char* in_row = static_cast<const char*>(p.logits) + row * p.row_stride * (IN == CBK_F32 ? 4 : 2);
     // offset of the thread's vector k of batch b: neighbouring lanes on neighbouring vectors
     auto offset = [&](int b, int k) { return ((b * kBatch + k) * kLgThreads + tid) * VEC; };
@@ -165,37 +231,39 @@ process_logits_kernel(const LogitsParams p) {
     };
     load_batch(0);
 
-    if (p.counted) {
-      if (turn == 0 || !p.shared) {
-        for (int i = tid; i < p.seg / 4; i += kLgThreads) reinterpret_cast<uint4*>(s_count)[i] = make_uint4(0, 0, 0, 0);
-        cluster_sync_all();                          // every CTA's counts are zero before any is added to
-        if (p.history) {
-          int64_t len = p.lengths ? p.lengths[row * p.len_stride] : p.hist_cap;
-          const int64_t prompt = p.n_prompt ? p.n_prompt[row * p.prompt_stride] : 0;
-          if (len < 0 || len > p.hist_cap) {
-            if (tid == 0) report(p.status, CBK_STATUS_BAD_INDEX);
-            len = len < 0 ? 0 : p.hist_cap;
-          }
-          const int64_t* h = p.history + row * p.hist_stride;
-          constexpr int kAhead = 8;
-          for (int64_t i = tid; i < len; i += kAhead * kLgThreads) {
-            int64_t t[kAhead];
+    for (int j = tid; j < p.n_tree; j += kLgThreads)
+      if ((p.tree_words[row * p.tree_stride + j / 32] >> (j % 32)) & 1u) {
+        const int64_t t = p.tree_tokens[j];
+        if (!ours(t) || !known(t)) continue;
+        const int o = offset_of(static_cast<uint32_t>(t));
+        s_path[atomicAdd(&s_n_path, 1)] = o;
+        atomicOr(s_over + o / 256, 1u << (o / 8 % 32));
+      }
+    if (counts_here && (turn == 0 || !p.shared)) {
+      for (int i = tid; i < p.seg / 4; i += kLgThreads) reinterpret_cast<uint4*>(s_count)[i] = make_uint4(0, 0, 0, 0);
+      int64_t len = p.lengths ? p.lengths[row * p.len_stride] : p.hist_cap;
+      const int64_t prompt = p.n_prompt ? p.n_prompt[row * p.prompt_stride] : 0;
+      if (len < 0 || len > p.hist_cap) {
+        if (rank == 0 && tid == 0) report(p.status, CBK_STATUS_BAD_INDEX);
+        len = len < 0 ? 0 : p.hist_cap;
+      }
+      const int64_t* h = p.history + row * p.hist_stride;
+      __syncthreads();
+      constexpr int kAhead = 8;
+      for (int64_t i = tid; i < len; i += kAhead * kLgThreads) {
+        int64_t t[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) t[k] = i + k * kLgThreads < len ? __ldg(h + i + k * kLgThreads) : 0;
+        for (int k = 0; k < kAhead; ++k) t[k] = i + k * kLgThreads < len ? __ldg(h + i + k * kLgThreads) : 0;
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k)
-              if (i + k * kLgThreads < len) add(t[k], i + k * kLgThreads >= prompt, 1u);
-          }
-        }
-        add_path(row, 1u);
-      } else {
-        // the last row's reads of the counts lie behind its closing cluster barrier
-        add_path(row - n_clusters, 0xffffffffu);
-        add_path(row, 1u);
+        for (int k = 0; k < kAhead; ++k)
+          if (i + k * kLgThreads < len && ours(t[k])) add(t[k], i + k * kLgThreads >= prompt);
       }
     }
-    // counts are whole; and every CTA of the cluster runs before one stores into rank 0
-    cluster_sync_all();
+    // a programmatic dependent of count_tokens_kernel: its counts are whole
+    if (p.counts && turn == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+    __syncthreads();
+    // every CTA of the cluster runs before one stores into rank 0
+    if (turn == 0) cluster_sync_all();
 
     float best = -INFINITY;
     int best_i = token_at(tid * VEC);                     // the thread's first element: the first of a row of -inf
@@ -205,7 +273,7 @@ process_logits_kernel(const LogitsParams p) {
     };
     auto penalise = [&](float x, uint32_t n) {
       if (n) {
-        x = x > 0.f ? __fdiv_rn(x, p.repetition) : __fmul_rn(x, p.repetition);
+        x = x > 0.f ? divide(x, p.repetition, p.inv_repetition) : __fmul_rn(x, p.repetition);
         const uint32_t c = n & ~kLgPrompt;
         if (c) x = __fsub_rn(__fsub_rn(x, __fmul_rn(p.frequency, static_cast<float>(c))), p.presence);
       }
@@ -217,6 +285,8 @@ process_logits_kernel(const LogitsParams p) {
         best_i = i;
       }
     };
+    const int n_path = p.n_tree > 0 ? s_n_path : 0;
+    auto on_path = [&](int o) { return n_path > 0 && ((s_over[o / 256] >> (o / 8 % 32)) & 1u); };
     const int n_batches = (p.seg + kBatch * kLgThreads * VEC - 1) / (kBatch * kLgThreads * VEC);
     for (int b = 0; b < n_batches; ++b) {
       if (b > 0) load_batch(b);
@@ -228,16 +298,26 @@ process_logits_kernel(const LogitsParams p) {
           float x[VEC];
 #pragma unroll
           for (int e = 0; e < VEC; ++e) x[e] = raw[k].at(e);
-          if (p.counted) {
+          if (p.history || n_path > 0) {
             uint32_t n[VEC], any = 0;
 #pragma unroll
             for (int q = 0; q < VEC / 4; ++q) {
-              const uint4 c4 = *reinterpret_cast<const uint4*>(s_count + o + 4 * q);
+              uint4 c4 = make_uint4(0, 0, 0, 0);
+              if (p.counts) c4 = *reinterpret_cast<const uint4*>(p.counts + i + 4 * q);
+              else if (p.history) c4 = *reinterpret_cast<const uint4*>(s_count + o + 4 * q);
               n[4 * q] = c4.x;
               n[4 * q + 1] = c4.y;
               n[4 * q + 2] = c4.z;
               n[4 * q + 3] = c4.w;
               any |= c4.x | c4.y | c4.z | c4.w;
+            }
+            if (on_path(o)) {
+              any = 1;
+              for (int j = 0; j < n_path; ++j) {
+                const int at = static_cast<int>(s_path[j]) - o;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) n[e] += at == e ? 1u : 0u;
+              }
             }
             if (any) {
 #pragma unroll
@@ -264,7 +344,13 @@ process_logits_kernel(const LogitsParams p) {
           float m = x[0];
 #pragma unroll
           for (int e = 1; e < VEC; ++e) m = max_nan(m, x[e]);
-          if (!(m <= best)) {                        // larger, or NaN: rare after the first few
+          if (m > best) {                            // the lowest of the equal ones
+            int at = VEC - 1;
+#pragma unroll
+            for (int e = VEC - 2; e >= 0; --e) at = x[e] == m ? e : at;
+            best = m;
+            best_i = i + at;
+          } else if (m != m) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) take(x[e], i + e);
           }
@@ -283,7 +369,10 @@ process_logits_kernel(const LogitsParams p) {
           // a row's last, partial vector, or a row off the boundaries
           for (int j = i; j < min(i + VEC, p.vocab); ++j) {
             float x = VEC == 1 ? raw[k].at(0) : load1<IN>(in_row, j);
-            if (p.counted) x = penalise(x, s_count[o + j - i]);
+            uint32_t n = p.counts ? p.counts[j] : p.history ? s_count[o + j - i] : 0u;
+            if (on_path(o + j - i))
+              for (int q = 0; q < n_path; ++q) n += static_cast<int>(s_path[q]) == o + j - i ? 1u : 0u;
+            x = penalise(x, n);
             if (p.bias) x = __fadd_rn(x, p.bias[row * p.bias_stride + j]);
             x = finish(x, j);
             take(x, j);
@@ -314,34 +403,54 @@ process_logits_kernel(const LogitsParams p) {
         asm volatile("st.relaxed.cluster.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(key) : "memory");
       }
     }
+    if (p.n_tree > 0) {                              // (the path's readers are behind the barrier above)
+      for (int j = tid; j < n_path; j += kLgThreads) s_over[s_path[j] / 256] = 0;
+      __syncthreads();
+      if (tid == 0) s_n_path = 0;
+    }
     cluster_sync_all();
     if (rank == 0 && tid == 0) {
       key = s_row[0];
-      for (int c = 1; c < kLgCluster; ++c) key = s_row[c] > key ? s_row[c] : key;
+      for (int c = 1; c <= cluster_mask; ++c) key = s_row[c] > key ? s_row[c] : key;
       p.tokens[row] = 0xffffffffu - static_cast<uint32_t>(key);
     }
+    if (row + n_clusters < p.rows) cluster_sync_all();   // read before the next row's choices arrive
   }
 }
 
 template <int IN, int OUT, int VEC>
 static int launch_logits(const LogitsParams& p, cudaStream_t st) {
   auto kern = process_logits_kernel<IN, OUT, VEC>;
-  const int smem = p.counted ? p.seg * 4 : 0;
-  if (smem > 48 * 1024)
-    if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), 224 * 1024)) return rc;
+  const int smem = ((p.history && !p.counts ? p.seg : 0) + (p.n_tree > 0 ? (p.seg + 255) / 256 + p.n_tree : 0)) * 4;
+  if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kLgMaxSmem)) return rc;
+  if (p.log_cluster > 3) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return set_error(CBK_ERR_CUDA, "process_logits_kernel: %s", cudaGetErrorString(e));
+  }
   cudaLaunchConfig_t cfg = {};
-  const int turns = (p.rows + kLgMaxClusters - 1) / kLgMaxClusters;      // rows per cluster
-  cfg.gridDim = dim3(static_cast<unsigned>((p.rows + turns - 1) / turns) * kLgCluster);
-  cfg.blockDim = dim3(kLgThreads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kLgCluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  if (p.counts) {
+    attr[0].val.clusterDim.x = kLgCountCtas;
+    cfg.gridDim = dim3(kLgCountCtas);
+    cfg.blockDim = dim3(1024);
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, count_tokens_kernel, p);
+    if (e != cudaSuccess) return set_error(CBK_ERR_CUDA, "count_tokens_kernel launch: %s", cudaGetErrorString(e));
+  }
+  const int fit = p.log_cluster == 2 ? kLgFit4 : kLgFit8;
+  const int turns = (p.rows + fit - 1) / fit, clusters = (p.rows + turns - 1) / turns;
+  attr[0].val.clusterDim.x = 1u << p.log_cluster;
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters) << p.log_cluster);
+  cfg.blockDim = dim3(kLgThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.numAttrs = p.counts ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) return set_error(CBK_ERR_CUDA, "process_logits_kernel launch: %s", cudaGetErrorString(e));
   return check_launch("process_logits_kernel");
@@ -350,6 +459,16 @@ static int launch_logits(const LogitsParams& p, cudaStream_t st) {
 }  // namespace cbk
 
 using namespace cbk;
+
+// many rows of one history: the counts live in the workspace
+static bool counted_once(int64_t rows, int64_t history_stride, int64_t lengths_stride, int64_t n_prompt_stride) {
+  return rows >= kLgManyRows && history_stride == 0 && lengths_stride == 0 && n_prompt_stride == 0;
+}
+
+extern "C" size_t cbk_process_logits_workspace_bytes(int64_t rows, int64_t vocab) {
+  if (rows < kLgManyRows || vocab <= 0 || vocab > kLgMaxVocab) return 0;
+  return static_cast<size_t>((vocab + 127) / 128 * 128) * sizeof(uint32_t);
+}
 
 extern "C" int cbk_process_logits(const cbk_process_logits_args* a, void* stream) {
   if (!a || a->size != sizeof(*a)) return set_error(CBK_ERR_INVALID, "cbk_process_logits: bad argument struct");
@@ -375,10 +494,22 @@ extern "C" int cbk_process_logits(const cbk_process_logits_args* a, void* stream
   if (a->history_cap < 0 || a->history_cap >= (int64_t{1} << 30) || a->n_tree < 0 || a->n_tree > 1024 ||
       (a->n_tree > 0 && (!a->tree_tokens || !a->tree_words || a->tree_stride < (a->n_tree + 31) / 32)))
     return set_error(CBK_ERR_INVALID, "cbk_process_logits: bad history or tree");
+  const bool history = a->history && a->history_cap > 0;
+  const bool shared = a->history_stride == 0 && a->lengths_stride == 0 && a->n_prompt_stride == 0;
+  const bool once = history && counted_once(a->rows, a->history_stride, a->lengths_stride, a->n_prompt_stride);
+  if (once) {
+    const size_t need = cbk_process_logits_workspace_bytes(a->rows, a->vocab);
+    if (a->workspace_bytes < 0 || static_cast<size_t>(a->workspace_bytes) < need)
+      return set_error(CBK_ERR_WORKSPACE, "cbk_process_logits: workspace %lld < %zu bytes",
+                       (long long)a->workspace_bytes, need);
+    if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 15u))
+      return set_error(CBK_ERR_INVALID, "cbk_process_logits: the workspace must be 16-byte aligned");
+  }
   LogitsParams p;
+  p.counts = once ? static_cast<uint32_t*>(a->workspace) : nullptr;
   p.logits = a->logits;
   p.out = a->out;
-  p.history = a->history_cap > 0 ? a->history : nullptr;
+  p.history = history ? a->history : nullptr;
   p.lengths = a->lengths;
   p.n_prompt = a->n_prompt;
   p.tree_tokens = a->tree_tokens;
@@ -398,11 +529,16 @@ extern "C" int cbk_process_logits(const cbk_process_logits_args* a, void* stream
   p.tree_stride = a->tree_stride;
   p.rows = static_cast<int>(a->rows);
   p.vocab = static_cast<int>(a->vocab);
-  p.seg = static_cast<int>((a->vocab + kLgCluster * kLgBlock - 1) / (kLgCluster * kLgBlock) * kLgBlock);
+  // clusters of 8 CTAs while all fit side by side, else, with no counts in shared
+  // memory, of 4; of 16 where the counts of a large vocabulary would not fit
+  p.log_cluster = p.rows > kLgFit8 && (once || !history) ? 2 : 3;
+  if (history && !once && (p.vocab / 8 + kLgBlock) * 4 + (p.vocab / 2048 + 2 + kLgMaxTree) * 4 > kLgMaxSmem) p.log_cluster = 4;
+  const int span = kLgBlock << p.log_cluster;
+  p.seg = (p.vocab + span - 1) / span * kLgBlock;
   p.n_tree = a->n_tree;
-  p.counted = p.history != nullptr || a->n_tree > 0;
-  p.shared = p.history == nullptr || (a->history_stride == 0 && a->lengths_stride == 0 && a->n_prompt_stride == 0);
+  p.shared = shared;
   p.repetition = a->repetition;
+  p.inv_repetition = static_cast<float>(1.0 / static_cast<double>(a->repetition));
   p.presence = a->presence;
   p.frequency = a->frequency;
   auto st = static_cast<cudaStream_t>(stream);

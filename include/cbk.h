@@ -337,7 +337,12 @@ int cbk_tree_attn(const cbk_tree_attn_args* args, void* stream);
  * no prompt, no bias, no mask.  in_dtype CBK_BF16 / CBK_F16 / CBK_F32; out_dtype
  * the same or CBK_F32.  A token outside [0, vocab) is skipped and a length
  * outside [0, history_cap] clamped, both with CBK_STATUS_BAD_INDEX.
- * vocab <= 458752, history_cap < 2^30, n_tree <= 1024, repetition > 0. */
+ * vocab <= 458752, history_cap < 2^30, n_tree <= 1024, repetition > 0.  Rows that
+ * share a history (history, lengths and n_prompt of stride 0) need, when there are
+ * many of them, a workspace for its counts: cbk_process_logits_workspace_bytes is 0
+ * when not.  16-byte aligned, no initialisation; calls that overlap on the GPU must
+ * not share it. */
+size_t cbk_process_logits_workspace_bytes(int64_t rows, int64_t vocab);
 typedef struct {
   int64_t size;                                  /* sizeof(cbk_process_logits_args) */
   const void* logits;
@@ -349,8 +354,9 @@ typedef struct {
   void* out;
   int64_t* tokens;
   int32_t* status;
+  void* workspace;
   int64_t row_stride, rows, vocab, history_stride, history_cap, lengths_stride, n_prompt_stride, bias_stride,
-      mask_stride, tree_stride, out_stride;
+      mask_stride, tree_stride, out_stride, workspace_bytes;
   int32_t n_tree, in_dtype, out_dtype;
   float repetition, presence, frequency;
 } cbk_process_logits_args;

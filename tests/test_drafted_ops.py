@@ -9,8 +9,8 @@ NR = dict(q=16, k=16, v=16, pos=16, rows=16, qw=16, kw=16, table=16, q_out=16, k
           vs=128, kvs=128, n=4, t_rows=10, cap=10, hq=4, hkv=2, d=64, r=64, il=0, dt=0, mode=1, eps=1e-6)
 TA = dict(q=16, k=16, v=16, n_ctx=16, words=16, out=16, ws=256, st=0, kvs=128, ws_=1, cap=100, bytes_=1 << 40, t=4,
           hq=4, hkv=2, d=64, dt=0, scale=0.1)
-PL = dict(x=16, h=16, ln=0, np_=0, bias=0, mask=0, tt=0, tw=0, out=16, tok=16, st=0, xs=100, rows=2, vocab=100, hs=0,
-          hc=5, ls=0, nps=0, bs=0, ms=0, ts=0, os=100, nt=0, dt=0, odt=2, rep=1.1, pres=0.0, freq=0.0)
+PL = dict(x=16, h=16, ln=0, np_=0, bias=0, mask=0, tt=0, tw=0, out=16, tok=16, st=0, ws=16, xs=100, rows=2, vocab=100, hs=0,
+          hc=5, ls=0, nps=0, bs=0, ms=0, ts=0, os=100, wb=0, nt=0, dt=0, odt=2, rep=1.1, pres=0.0, freq=0.0)
 
 
 def call(name, fields, **change):
@@ -64,7 +64,8 @@ def test_tree_attn_workspace_refusals():
     (dict(rows=-1), -1), (dict(x=0), -1), (dict(tok=0), -1), (dict(rep=0.0), -1), (dict(rep=-1.0), -1),
     (dict(rep=float("nan")), -1), (dict(pres=float("nan")), -1), (dict(xs=99), -1), (dict(os=99), -1),
     (dict(mask=16, ms=3), -1), (dict(bias=16, bs=99), -1), (dict(hc=-1), -1), (dict(nt=2), -1), (dict(nt=1025), -1),
-    (dict(nt=33, tt=16, tw=16, ts=1), -1), (dict(rows=0), 0),
+    (dict(nt=33, tt=16, tw=16, ts=1), -1), (dict(rows=64, wb=511), -4), (dict(rows=64, ws=0, wb=512), -1),
+    (dict(rows=64, ws=8, wb=512), -1), (dict(rows=0), 0),
 ])
 def test_process_logits_refusals(change, code):
     assert call("process_logits", PL, **change) == code
