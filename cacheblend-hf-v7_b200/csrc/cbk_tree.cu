@@ -96,6 +96,11 @@ __device__ __forceinline__ uint32_t tree_bits(const uint32_t* w, int n, int off)
   return __funnelshift_r(word(off >> 5), word((off >> 5) + 1), off & 31);
 }
 
+// 16 bytes from global to shared memory, asynchronously; zeros when not `there`
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
 template <int HD, int NQ, int NST>
 struct TreeSmem {
   static constexpr int kQBytes = kBM * HD * 2;
@@ -194,25 +199,17 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   } else if (warp >= 4) {
     // Q tiles in the layout a 128-byte-swizzled TMA copy leaves: 16-byte piece c of
     // row r at piece c ^ (r & 7); rows that do not exist are zero
-    constexpr int kVec = HD / 8, kStep = (kTreeThreads - 128) / kVec, kAhead = kBM / kStep;
-    const int c = threadIdx.x % kVec, r0 = (threadIdx.x - 128) / kVec;
-    const int row0 = 2 * pair * kBM;
-    for (int r = r0; r < (two ? 2 : 1) * kBM; r += kStep * kAhead) {
-      uint4 x[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int row = row0 + r + k * kStep, node = row / p.group;
-        x[k] = make_uint4(0, 0, 0, 0);
-        if (row < p.rows)
-          x[k] = ld_vec(p.q + (static_cast<int64_t>(node) * p.n_q + kvh * p.group + row - node * p.group) * HD + c * 8);
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int at = r + k * kStep;
-        *reinterpret_cast<uint4*>(sbase + (at / kBM) * L::kQBytes + (c >> 3) * (kBM * 128) + (at % kBM) * 128 +
-                                  ((c ^ at) & 7) * 16) = x[k];
-      }
+    constexpr int kVec = HD / 8, kStep = (kTreeThreads - 128) / kVec;
+    const int c = threadIdx.x % kVec, row0 = 2 * pair * kBM;
+    const int n_rows = (two ? 2 : 1) * kBM;
+#pragma unroll 8
+    for (int r = (threadIdx.x - 128) / kVec; r < n_rows; r += kStep) {
+      const int row = min(row0 + r, p.rows - 1), node = row / p.group;
+      cp_async16_or_zero(base + (r / kBM) * L::kQBytes + (c >> 3) * (kBM * 128) + (r % kBM) * 128 + ((c ^ r) & 7) * 16,
+                         p.q + (static_cast<int64_t>(node) * p.n_q + kvh * p.group + row - node * p.group) * HD + c * 8,
+                         row0 + r < p.rows);
     }
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
     fence_proxy_async_smem();
   }
   tc_fence_before();
@@ -545,13 +542,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 }
 
 // Merge of the splits, a warp per query row: O = sum_i w_i O_i / sum_i w_i l_i,
-// w_i = 2^(m_i - M) over the splits that hold a key tile, in their order, eight O
+// w_i = 2^(m_i - M) over the splits that hold a key tile, in their order, sixteen O
 // loads in flight.  A row that sees nothing has every l_i = 0 and gets zeros.
 // (With one such split the attention kernel has written the output.)
 template <int DT, int HD>
 __global__ void __launch_bounds__(kTreeMergeWarps * 32)
 tree_merge_kernel(const TreeParams p, int n_kv) {
-  constexpr int kD = HD / 32, kAhead = 8;
+  constexpr int kD = HD / 32, kAhead = 16;
   using Vec = typename std::conditional<kD == 4, float4, float2>::type;
   __shared__ float s_w[kTreeMergeWarps][kTreeMaxSplits];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
