@@ -8,6 +8,7 @@ an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Sequence
 
 import numpy as np
@@ -613,7 +614,7 @@ def norm_rope_scatter(q_src: torch.Tensor, k_src: torch.Tensor, v_src: torch.Ten
     elif q_weight is not None or k_weight is not None:
         raise ValueError("norm_rope_scatter: give both q_weight and k_weight, or neither")
     if q_out is None:
-        q_out = q2.new_empty((n, qd))
+        q_out = torch.empty_like(q2, memory_format=torch.contiguous_format)
     elif q_out.dtype != dt or q_out.numel() != n * qd or not q_out.is_contiguous():
         raise ValueError(f"norm_rope_scatter: q_out must be contiguous {dt} with {n} rows of {qd}")
     _norm_rope_scatter(dev, q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), positions.data_ptr(), rows.data_ptr(), qw, kw,
@@ -623,20 +624,25 @@ def norm_rope_scatter(q_src: torch.Tensor, k_src: torch.Tensor, v_src: torch.Ten
     return q_out
 
 
+@functools.lru_cache(maxsize=1024)
+def _tree_workspace_bytes(n_nodes: int, cap: int, n_q_heads: int, n_kv_heads: int, head_dim: int, index: int) -> int:
+    """Workspace size on device ``index`` (it goes by that device's SMs)."""
+    if head_dim not in (64, 128) or n_nodes > 1024:
+        raise NotImplementedError(f"tree_attn: head_dim 64 or 128 and at most 1024 nodes, got {head_dim}, {n_nodes}")
+    with torch.cuda.device(index):
+        nbytes = N.LIB.cbk_tree_attn_workspace_bytes(n_nodes, cap, n_q_heads, n_kv_heads, head_dim)
+    if nbytes == 0:
+        raise ValueError(f"tree_workspace: {N.last_error()}")
+    return nbytes
+
+
 def tree_workspace(n_nodes: int, cap: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
     """Workspace of tree_attn for up to n_nodes nodes over a cache of cap rows
     (reusable by calls that do not overlap on the GPU)."""
-    if head_dim not in (64, 128) or n_nodes > 1024:
-        raise NotImplementedError(f"tree_attn: head_dim 64 or 128 and at most 1024 nodes, got {head_dim}, {n_nodes}")
     device = torch.device(device)
-    if device.index is None or torch.cuda.current_device() == device.index:
-        nbytes = N.LIB.cbk_tree_attn_workspace_bytes(n_nodes, cap, n_q_heads, n_kv_heads, head_dim)
-    else:
-        with torch.cuda.device(device):          # sized for that device's SMs
-            nbytes = N.LIB.cbk_tree_attn_workspace_bytes(n_nodes, cap, n_q_heads, n_kv_heads, head_dim)
-    if nbytes == 0:
-        raise ValueError(f"tree_workspace: {N.last_error()}")
-    return torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    nbytes = _tree_workspace_bytes(n_nodes, cap, n_q_heads, n_kv_heads, head_dim, index)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_ctx: torch.Tensor,
@@ -668,11 +674,12 @@ def tree_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_c
         q = q.clone(memory_format=torch.contiguous_format)
     words, words_stride = _word_rows(words)
     if workspace is None:
-        workspace = tree_workspace(t, cap, n_q_heads, n_kv_heads, head_dim, dev)
+        workspace = torch.empty(_tree_workspace_bytes(t, cap, n_q_heads, n_kv_heads, head_dim, dev.index),
+                                dtype=torch.uint8, device=dev)
     elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise ValueError("tree_attn: workspace must come from tree_workspace")
     if out is None:
-        out = torch.empty_like(q).view(t, qd) if q.dim() != 2 else torch.empty_like(q)
+        out = torch.empty_like(q) if q.dim() == 2 else torch.empty_like(q).view(t, qd)
     elif out.dtype != dt or out.numel() != t * qd or not out.is_contiguous():
         raise ValueError(f"tree_attn: out must be contiguous {dt} with {t} rows of {qd}")
     _tree_attn(dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), n_ctx.data_ptr(), words.data_ptr(),
@@ -824,11 +831,13 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, le
             raise ValueError("process_logits: out rows must be contiguous")
         out_p, out_code = out2.data_ptr(), _DT3.get(out.dtype)
     elif return_logits:
-        out = logits.new_empty(shape) if out_dtype is None else logits.new_empty(shape, dtype=out_dtype)
+        out = torch.empty_like(logits, dtype=out_dtype, memory_format=torch.contiguous_format)
+        if not flat:
+            out = out.view(shape)
         out_p, out_code, out_stride = out.data_ptr(), _DT3.get(out.dtype), vocab
     if out_code is None:
         raise NotImplementedError(f"process_logits: bf16, fp16 or fp32 output, got {out.dtype}")
-    tokens = torch.empty(shape[:-1], dtype=torch.int64, device=dev)
+    tokens = torch.empty(rows if flat else shape[:-1], dtype=torch.int64, device=dev)
     if not (repetition > 0 and presence == presence and frequency == frequency):
         raise ValueError("process_logits: repetition must be > 0 and no penalty NaN")
     if repetition == 1.0 and presence == 0.0 and frequency == 0.0:
