@@ -36,8 +36,8 @@ class _Choice:
                  allowed_tokens: torch.Tensor | None, status: torch.Tensor | None):
         self.penalties = dict(repetition=float(repetition_penalty), presence=float(presence_penalty),
                               frequency=float(frequency_penalty))
-        if not repetition_penalty > 0:
-            raise ValueError(f"repetition_penalty must be > 0, got {repetition_penalty}")
+        if not 0 < repetition_penalty < float("inf"):
+            raise ValueError(f"repetition_penalty must be positive and finite, got {repetition_penalty}")
         self.counted = (repetition_penalty, presence_penalty, frequency_penalty) != (1.0, 0.0, 0.0)
         self.status = status
         self.bias = self.mask = None

@@ -576,7 +576,7 @@ def norm_rope_scatter(q_src: torch.Tensor, k_src: torch.Tensor, v_src: torch.Ten
     [n][Hq*D].
 
     q_src / k_src / v_src: n rows of heads (views of one stacked projection are
-    read in place); ``positions`` and ``rows``: int64, n entries -- siblings of a
+    read in place; q_out must not overlap them); ``positions`` and ``rows``: int64, n entries -- siblings of a
     drafted tree share a position, not a row; rows are distinct, and a row of -1
     marks a padding token of which nothing is written.  ``rope``: fp32 (cos, sin)
     table [n_pos][R / 2][2]; the first R dimensions of a head are rotated, as the
@@ -838,8 +838,8 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None, le
     if out_code is None:
         raise NotImplementedError(f"process_logits: bf16, fp16 or fp32 output, got {out.dtype}")
     tokens = torch.empty(rows if flat else shape[:-1], dtype=torch.int64, device=dev)
-    if not (repetition > 0 and presence == presence and frequency == frequency):
-        raise ValueError("process_logits: repetition must be > 0 and no penalty NaN")
+    if not (0 < repetition < float("inf") and presence == presence and frequency == frequency):
+        raise ValueError("process_logits: repetition must be positive and finite, and no penalty NaN")
     if repetition == 1.0 and presence == 0.0 and frequency == 0.0:
         hist_cap = n_tree = 0                    # nothing depends on the counts
     ws = ws_bytes = 0

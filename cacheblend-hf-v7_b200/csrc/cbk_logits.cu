@@ -93,13 +93,16 @@ __device__ __forceinline__ void store1(void* p, int64_t i, float x) {
   else static_cast<uint16_t*>(p)[i] = Elem<DT>::from_f(x);
 }
 
-// x / b for x > 0, correctly rounded, from y = the rounded 1 / b: with q = RN(x y), the
-// remainder r = x - q b is exact in one FMA, and RN(q + r y) is the rounded quotient
-// (Markstein, "Computation of elementary functions on the IBM RISC System/6000
-// processor", 1990) as long as nothing under- or overflows on the way.
+// x / b for x > 0, correctly rounded, from y = the rounded 1 / b: q = RN(x y) is
+// within two units of the quotient, one correction by its exact remainder brings it
+// within one, and then RN(q + (x - q b) y) is the rounded quotient (Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor", 1990)
+// as long as nothing under- or overflows on the way: y = 0 where b is not between
+// 2^-40 and 2^40, and then, or for x outside the range below, the division itself.
 __device__ __forceinline__ float divide(float x, float b, float y) {
-  if (!(x > 1e-20f && x < 1e20f)) return __fdiv_rn(x, b);
-  const float q = __fmul_rn(x, y);
+  if (!(x > 1e-20f && x < 1e20f) || y == 0.f) return __fdiv_rn(x, b);
+  float q = __fmul_rn(x, y);
+  q = __fmaf_rn(__fmaf_rn(-q, b, x), y, q);
   return __fmaf_rn(__fmaf_rn(-q, b, x), y, q);
 }
 
@@ -484,7 +487,8 @@ extern "C" int cbk_process_logits(const cbk_process_logits_args* a, void* stream
     return set_error(CBK_ERR_INVALID, "cbk_process_logits: %lld rows", (long long)a->rows);
   if (a->rows == 0) return CBK_OK;
   if (!a->logits || !a->tokens) return set_error(CBK_ERR_INVALID, "cbk_process_logits: null pointer argument");
-  if (!(a->repetition > 0.f)) return set_error(CBK_ERR_INVALID, "cbk_process_logits: repetition penalty must be > 0");
+  if (!(a->repetition > 0.f && a->repetition < INFINITY))
+    return set_error(CBK_ERR_INVALID, "cbk_process_logits: repetition penalty must be positive and finite");
   if (a->presence != a->presence || a->frequency != a->frequency)
     return set_error(CBK_ERR_INVALID, "cbk_process_logits: presence / frequency penalty is NaN");
   if (a->row_stride < a->vocab || (a->out && a->out_stride < a->vocab) ||
@@ -538,7 +542,8 @@ extern "C" int cbk_process_logits(const cbk_process_logits_args* a, void* stream
   p.n_tree = a->n_tree;
   p.shared = shared;
   p.repetition = a->repetition;
-  p.inv_repetition = static_cast<float>(1.0 / static_cast<double>(a->repetition));
+  p.inv_repetition = a->repetition >= 0x1p-40f && a->repetition <= 0x1p40f
+      ? static_cast<float>(1.0 / static_cast<double>(a->repetition)) : 0.f;
   p.presence = a->presence;
   p.frequency = a->frequency;
   auto st = static_cast<cudaStream_t>(stream);

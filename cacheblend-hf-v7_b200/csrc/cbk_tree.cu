@@ -634,9 +634,10 @@ static TreeLayout tree_layout(int n_nodes, int64_t cap, int n_q_heads, int n_kv_
   const int64_t sms = std::min(attn_sm_count(), kTreeMaxSplits);
   t.n_splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / units, (cap + kBN - 1) / kBN)));
   t.row_pitch = (std::min(t.rows, kBM) + 7) / 8 * 8;
-  const size_t slots = static_cast<size_t>(units) * t.n_splits * (t.n_qt == 1 ? 1 : 2);
+  // one split writes the output itself
+  const size_t slots = t.n_splits == 1 ? 0 : static_cast<size_t>(units) * t.n_splits * (t.n_qt == 1 ? 1 : 2);
   t.off_o = (slots * t.row_pitch * sizeof(float2) + 255) & ~static_cast<size_t>(255);
-  t.bytes = t.off_o + slots * t.row_pitch * head_dim * sizeof(float);
+  t.bytes = std::max<size_t>(256, t.off_o + slots * t.row_pitch * head_dim * sizeof(float));
   return t;
 }
 
@@ -651,6 +652,7 @@ static int launch_tree(const cbk_tree_attn_args* a, const TreeParams& p, cudaStr
   if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem)) return rc;
   kern<<<dim3(p.n_splits, a->n_kv_heads, p.n_pairs), kTreeThreads, smem, st>>>(mk, mv, p);
   if (int rc = check_launch("tree_attn_kernel")) return rc;
+  if (p.n_splits == 1) return CBK_OK;
   cudaLaunchConfig_t cfg = {};
   const int64_t rows = static_cast<int64_t>(a->n_kv_heads) * p.rows;
   cfg.gridDim = dim3(static_cast<unsigned>((rows + kTreeMergeWarps - 1) / kTreeMergeWarps));

@@ -337,7 +337,8 @@ int cbk_tree_attn(const cbk_tree_attn_args* args, void* stream);
  * no prompt, no bias, no mask.  in_dtype CBK_BF16 / CBK_F16 / CBK_F32; out_dtype
  * the same or CBK_F32.  A token outside [0, vocab) is skipped and a length
  * outside [0, history_cap] clamped, both with CBK_STATUS_BAD_INDEX.
- * vocab <= 458752, history_cap < 2^30, n_tree <= 1024, repetition > 0.  Rows that
+ * vocab <= 458752, history_cap < 2^30, n_tree <= 1024, repetition positive and
+ * finite.  Rows that
  * share a history (history, lengths and n_prompt of stride 0) need, when there are
  * many of them, a workspace for its counts: cbk_process_logits_workspace_bytes is 0
  * when not.  16-byte aligned, no initialisation; calls that overlap on the GPU must

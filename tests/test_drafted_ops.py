@@ -62,7 +62,7 @@ def test_tree_attn_workspace_refusals():
 @pytest.mark.parametrize("change,code", [
     (dict(dt=3), -2), (dict(odt=1), -2), (dict(dt=2, odt=0), -2), (dict(vocab=0), -2), (dict(vocab=1 << 20), -2),
     (dict(rows=-1), -1), (dict(x=0), -1), (dict(tok=0), -1), (dict(rep=0.0), -1), (dict(rep=-1.0), -1),
-    (dict(rep=float("nan")), -1), (dict(pres=float("nan")), -1), (dict(xs=99), -1), (dict(os=99), -1),
+    (dict(rep=float("nan")), -1), (dict(rep=float("inf")), -1), (dict(pres=float("nan")), -1), (dict(xs=99), -1), (dict(os=99), -1),
     (dict(mask=16, ms=3), -1), (dict(bias=16, bs=99), -1), (dict(hc=-1), -1), (dict(nt=2), -1), (dict(nt=1025), -1),
     (dict(nt=33, tt=16, tw=16, ts=1), -1), (dict(rows=64, wb=511), -4), (dict(rows=64, ws=0, wb=512), -1),
     (dict(rows=64, ws=8, wb=512), -1), (dict(rows=0), 0),

@@ -336,6 +336,53 @@ def test_tree_attn_captured_context_advances(ops):
         ta_check(out, q, k, v, n_ctx, words, hq, hkv, d, d ** -0.5)
 
 
+def on_gpu_check(got, q, k, v, n_ctx, words, hq, hkv, d, scale, heads=None):
+    """ta_check in 64 bits on the GPU, head by head (finite caches)."""
+    t, n = words.shape[0], n_ctx + words.shape[0]
+    sees = torch.ones((t, n), dtype=torch.bool, device=DEV)
+    sees[:, n_ctx:] = ref.visible(words, t).to(DEV)
+    for h in range(hq) if heads is None else heads:
+        at = slice(h // (hq // hkv) * d, (h // (hq // hkv) + 1) * d)
+        kk, vv = k[:n, at].to(DEV).double(), v[:n, at].to(DEV).double()
+        s = (q[:, h * d:(h + 1) * d].to(DEV).double() @ kk.T * scale).masked_fill(~sees, -torch.inf)
+        p = torch.softmax(s, 1).nan_to_num(0.0)              # (a row that sees nothing: zeros)
+        out, A = p @ vv, p @ vv.abs()
+        bound = ref.tree_bound(out, A, n, q.dtype, float(vv.abs().max()))
+        err = (got[:, h * d:(h + 1) * d].double() - out).abs()
+        assert (err <= bound).all(), (h, float((err / bound).max()))
+
+
+@pytest.mark.parametrize("t,n_ctx,hq,hkv,d,dt", [(1024, 300, 4, 1, 128, BF), (999, 0, 6, 2, 64, HF),
+                                                 (640, 5000, 3, 3, 128, BF)])
+def test_tree_attn_many_nodes(ops, t, n_ctx, hq, hkv, d, dt):
+    """Many Q tiles, odd counts of them, and key tiles of the tree alone."""
+    q, k, v, words, cap = ta_inputs(t, n_ctx, hq, hkv, d, dt, "sparse", spare=3)
+    got = ops.tree_attn(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor([n_ctx], device=DEV), words.to(DEV), hq, hkv, d,
+                        d ** -0.5)
+    on_gpu_check(got, q, k, v, n_ctx, words, hq, hkv, d, d ** -0.5)
+
+
+def test_offsets_past_32_bits(ops):
+    """A cache of more than 2^31 elements: rows written and read behind that."""
+    t, hq, hkv, d, n_ctx = 5, 8, 8, 128, 2_200_000
+    cap = n_ctx + t + 4
+    g = torch.Generator(device=DEV).manual_seed(4)
+    k = torch.randn((cap, hkv * d), generator=g, device=DEV, dtype=BF)
+    v = torch.randn((cap, hkv * d), generator=g, device=DEV, dtype=BF)
+    assert k.numel() > 2 ** 31
+    qkv, _, pos, w, _, _, tab = nr_inputs(t, hq, hkv, d, d, BF, True)
+    rows = n_ctx + torch.arange(t)
+    q = ops.norm_rope_scatter(*nr_split(qkv.to(DEV), hq, hkv, d), pos.to(DEV), rows.to(DEV), hq, hkv, d, tab.to(DEV), k, v,
+                              *[x.to(DEV) for x in w], mode="fp32")
+    z, mag = ref.norm_rope(nr_split(qkv, hq, hkv, d)[1], hkv, d, w[1], 1e-6, tab, pos, False)
+    assert ((k[rows.to(DEV)].cpu().double() - z).abs() <= ref.norm_rope_bound(z, mag, BF, "fp32")).all()
+    assert torch.equal(v[rows.to(DEV)].cpu(), nr_split(qkv, hq, hkv, d)[2])
+    q = q * 8                                           # peaked: single far rows count
+    words, _ = ops.tree_words([-1, 0, 0, 1, 2])
+    got = ops.tree_attn(q, k, v, torch.tensor([n_ctx], device=DEV), words.to(DEV), hq, hkv, d, d ** -0.5)
+    on_gpu_check(got, q, k, v, n_ctx, words, hq, hkv, d, d ** -0.5, heads=[0, 7])
+
+
 # ---------------------------------------------------------------------------
 # process_logits
 # ---------------------------------------------------------------------------
@@ -455,6 +502,54 @@ def test_process_logits_edges(ops):
     pl_check(ops, x, None, history=torch.zeros((1, 0), dtype=torch.int64), repetition=1.5)
 
 
+@pytest.mark.parametrize("rows,vocab,dt", [(24, 5000, BF), (31, 3001, HF), (67, 4096, BF), (150, 1000, torch.float32)])
+def test_process_logits_many_rows(ops, rows, vocab, dt):
+    """More rows than clusters: a shared history counted once, one per row, none, and a tree."""
+    x, h, g = pl_inputs(rows, vocab, 700, dt)
+    own = (torch.rand((rows, 90), generator=g) ** 3 * vocab).long().clamp_(max=vocab - 1)
+    n = torch.tensor([300])
+    mask = torch.randint(-2 ** 31, 2 ** 31, (rows, (vocab + 31) // 32), generator=g).to(torch.int32)
+    words, _ = ops.tree_words([-1] + [int(torch.randint(max(0, i - 3), i, (1,), generator=g)) for i in range(1, rows)])
+    toks = torch.randint(0, 60, (rows,), generator=g)
+    x[:, :60] += 6
+    kw = dict(repetition=1.15, presence=0.2, frequency=0.3)
+    assert pl_check(ops, x, torch.float32, history=h, n_prompt=n, mask_words=mask, **kw) == 0
+    assert pl_check(ops, x, None, history=h, lengths=n, tree_tokens=toks, tree_words=words, **kw) == 0
+    assert pl_check(ops, x, None, history=own, lengths=torch.randint(0, 91, (rows,), generator=g),
+                    tree_tokens=toks, tree_words=words, **kw) == 0
+    assert pl_check(ops, x, None, history=h, lengths=torch.randint(0, 701, (rows,), generator=g), **kw) == 0
+    assert pl_check(ops, x, None, tree_tokens=toks, tree_words=words, **kw) == 0
+    assert pl_check(ops, x, torch.float32, bias=torch.randn((vocab,), generator=g)) == 0
+
+
+def test_process_logits_offsets_past_32_bits(ops):
+    rows, vocab = 17000, 128256
+    g = torch.Generator(device=DEV).manual_seed(9)
+    x = torch.randn((rows, vocab), generator=g, device=DEV, dtype=BF)
+    assert x.numel() > 2 ** 31
+    h = torch.randint(0, vocab, (500,), generator=g, device=DEV)
+    out, tok = ops.process_logits(x, history=h, repetition=1.2, frequency=0.1)
+    at = torch.tensor([0, 65, 66, 16743, 16744, 16999], device=DEV)
+    exp, exp_tok = ref.logits(x[at], history=h, repetition=1.2, frequency=0.1)
+    assert torch.equal(out[at].cpu(), exp.to(BF)) and torch.equal(tok[at].cpu(), exp_tok)
+
+
+def test_process_logits_division_is_the_rounded_quotient(ops):
+    """x / repetition for many mantissas and exponents, penalties in and out of the
+    range of the fast way, to the bit."""
+    g = gen(17)
+    n = 1 << 18
+    x = (1 + torch.rand((1, n), generator=g, dtype=torch.float64)).float()
+    x[0, :9] = torch.tensor([1e-40, 1e-38, 9e-21, 1.1e-20, 1e20, 2e20, 3e38, float("inf"), 1.0])
+    x[0, 9:n // 2] *= torch.exp2(torch.randint(-30, 30, (n // 2 - 9,), generator=g).float())
+    x[0, n // 2:n // 2 + 1000] = 2 - torch.arange(1, 1001) * 2.0 ** -23          # mantissas near 2
+    h = torch.arange(n)
+    below_two = float(np.nextafter(np.float32(2), np.float32(0)))
+    for rep in (1.1, 1.3, 0.7, 3.0, below_two, float(np.nextafter(np.float32(1), np.float32(2))), 1.0 / 3, 1e-12, 1e11,
+                1e-20, 1e30, 3e-39):
+        pl_check(ops, x, None, history=h, repetition=rep, bias=torch.zeros(n))
+
+
 def test_process_logits_bad_tokens_are_skipped_and_reported(ops):
     x = torch.randn((2, 100), generator=gen(5)).to(BF)
     h = torch.tensor([[1, 2, -1, 100, 5], [7, 7, 1 << 40, 8, 9]])
@@ -462,6 +557,17 @@ def test_process_logits_bad_tokens_are_skipped_and_reported(ops):
     assert pl_check(ops, x, None, history=h[:, :2], lengths=torch.tensor([1, 9]), repetition=1.4) & 1
     assert pl_check(ops, x, None, history=h[:, :2], lengths=torch.tensor([-4, 2]), repetition=1.4) & 1
     assert pl_check(ops, x, None, history=h[:, :2], lengths=torch.tensor([1, 2]), repetition=1.4) == 0
+    # a tree's token outside the vocabulary, on one row's path; and with the history counted once
+    words = torch.tensor([[1], [3]], dtype=torch.int32)
+    st = status_word()
+    _, tok = ops.process_logits(x.to(DEV), tree_tokens=torch.tensor([5, 100], device=DEV), tree_words=words.to(DEV),
+                                repetition=1.4, status=st)
+    exp, exp_tok = ref.logits(x, tree_tokens=torch.tensor([5, 5]), tree_words=torch.ones_like(words), repetition=1.4)
+    assert int(st.item()) & 1 and torch.equal(tok.cpu(), exp_tok)
+    many = torch.randn((40, 100), generator=gen(6)).to(BF)
+    assert pl_check(ops, many, None, history=h[0], repetition=1.4, presence=0.3) & 1
+    assert pl_check(ops, many, None, history=h[0, :2], lengths=torch.tensor([9]), repetition=1.4) & 1
+    assert pl_check(ops, many, None, history=h[0, :2], repetition=1.4) == 0
 
 
 def test_process_logits_refusals(ops):
@@ -469,7 +575,7 @@ def test_process_logits_refusals(ops):
     h = torch.zeros((5,), dtype=torch.int64, device=DEV)
     for bad in (dict(lengths=h[:1]), dict(history=h.int()), dict(history=h.expand(3, 5)), dict(tree_tokens=h),
                 dict(history=h, lengths=h[:3]), dict(bias=x[0]), dict(bias=x.float()[:, :5]), dict(mask_words=h),
-                dict(mask_words=h[:1].int()), dict(repetition=0.0), dict(presence=float("nan")),
+                dict(mask_words=h[:1].int()), dict(repetition=0.0), dict(repetition=float("inf")), dict(presence=float("nan")),
                 dict(tree_tokens=h, tree_words=h.int().view(1, 5)), dict(out=x[:1]),
                 dict(out=x, out_dtype=torch.float32)):
         with pytest.raises(ValueError):
