@@ -20,6 +20,27 @@ namespace cbk {
 int set_error(int code, const char* fmt, ...);
 int check_launch(const char* what);
 
+// Launch as a programmatic dependent of the kernel before it in the stream: its
+// launch overlaps that kernel's end.  The kernel calls grid_wait() before it touches
+// global memory.
+template <typename... P, typename... A>
+inline int launch_dependent(const char* what, void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                            const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e != cudaSuccess) return set_error(CBK_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
+}
+
 // ---------------------------------------------------------------------------
 // 16-bit element traits
 // ---------------------------------------------------------------------------
@@ -114,6 +135,12 @@ __device__ __forceinline__ uint4 ld_vec(const void* p) {
 __device__ __forceinline__ void st_vec(void* p, uint4 v) {
   *reinterpret_cast<uint4*>(p) = v;
 }
+
+// Programmatic dependent launch: wait until the kernels before this one in the stream
+// are complete and their writes visible (a no-op in an ordinary launch).
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// ... and let the kernel after this one be placed as SMs free up; it waits by itself.
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
 
 __device__ __forceinline__ void report(int32_t* status, int bits) {
   if (status) atomicOr(status, bits);

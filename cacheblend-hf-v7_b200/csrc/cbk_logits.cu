@@ -177,7 +177,7 @@ count_tokens_kernel(const LogitsParams p) {
     }
   }
   if (bad) report(p.status, CBK_STATUS_BAD_INDEX);
-  asm volatile("griddepcontrol.launch_dependents;");
+  grid_launch_dependents();
 }
 
 template <int IN, int OUT, int VEC>
@@ -262,8 +262,7 @@ process_logits_kernel(const LogitsParams p) {
           if (i + k * kLgThreads < len && ours(t[k])) add(t[k], i + k * kLgThreads >= prompt);
       }
     }
-    // a programmatic dependent of count_tokens_kernel: its counts are whole
-    if (p.counts && turn == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (p.counts && turn == 0) grid_wait();          // a dependent of count_tokens_kernel: its counts are whole
     __syncthreads();
     // every CTA of the cluster runs before one stores into rank 0
     if (turn == 0) cluster_sync_all();

@@ -124,9 +124,13 @@ norm_rope_scatter_kernel(const NormRopeParams p) {
 #pragma unroll
     for (int i = 0; i < kNrSlots; ++i) mbar_init(bar0 + 8 * i, 1);
     fence_barrier_init();
+  }
+  grid_wait();
+  if (lane == 0) {
     for (int c = first; c < min(last, first + kNrSlots); ++c) fetch(c);
   }
   __syncwarp();
+  grid_launch_dependents();
   const int64_t pos = p.pos[j], row = p.rows[j];
   bool failed = false;
   auto landed = [&](int c) {
@@ -314,8 +318,8 @@ static int launch_norm_rope(NormRopeParams& p, int interleaved, int mode, cudaSt
                            : (interleaved ? norm_rope_scatter_kernel<DT, LPH, false, true>
                                           : norm_rope_scatter_kernel<DT, LPH, false, false>);
   if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kNrSmem)) return rc;
-  kern<<<static_cast<unsigned>(blocks), kNrThreads, kNrSmem, st>>>(p);
-  return check_launch("norm_rope_scatter_kernel");
+  return launch_dependent("norm_rope_scatter_kernel", kern, dim3(static_cast<unsigned>(blocks)), dim3(kNrThreads), kNrSmem,
+                          st, p);
 }
 
 template <int DT>

@@ -123,6 +123,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   enum { KFULL = 0, KEMPTY = NST, VFULL = 2 * NST, VEMPTY = 3 * NST, VCLEAN = 4 * NST, SFULL = 5 * NST,
          PHALF = SFULL + 2, PFULL = SFULL + 4, ODONE = SFULL + 6, DRAIN = SFULL + 8 };
   const int split = blockIdx.x, kvh = blockIdx.y, pair = blockIdx.z;
+  grid_wait();
   const TreeSpan sp = tree_span(p);
   if (!sp.ok) {
     if (threadIdx.x == 0 && split == 0 && kvh == 0 && pair == 0) report(p.status, CBK_STATUS_BAD_INDEX);
@@ -217,7 +218,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   // the merge kernel (a programmatic dependent) may be placed as SMs free up
-  asm volatile("griddepcontrol.launch_dependents;");
+  grid_launch_dependents();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -562,9 +563,10 @@ tree_merge_kernel(const TreeParams p, int n_kv) {
   const float2* ml = p.part_ml + slot0 * p.row_pitch + r;
   const float* po = p.part_o + (slot0 * p.row_pitch + r) * HD + lane * kD;
   const int64_t step = static_cast<int64_t>(per) * p.row_pitch;
-  // (n_ctx is no result of the attention kernel: whoever writes it is done)
+  // (n_ctx is no result of the attention kernel, which began once its writer was done)
   const TreeSpan sp = tree_span(p);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_wait();
+  grid_launch_dependents();
   if (!sp.ok) return;                                  // reported by the attention kernel
   const int n = min(sp.n_tiles, p.n_splits);           // splits 0 .. n - 1 hold key tiles
   if (n == 1) return;
@@ -650,22 +652,14 @@ static int launch_tree(const cbk_tree_attn_args* a, const TreeParams& p, cudaStr
   constexpr int smem = TreeSmem<HD, NQ, NST>::kAlloc;
   static_assert(smem <= 227 * 1024, "shared memory of tree_attn_kernel");
   if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem)) return rc;
-  kern<<<dim3(p.n_splits, a->n_kv_heads, p.n_pairs), kTreeThreads, smem, st>>>(mk, mv, p);
-  if (int rc = check_launch("tree_attn_kernel")) return rc;
+  if (int rc = launch_dependent("tree_attn_kernel", kern, dim3(p.n_splits, a->n_kv_heads, p.n_pairs),
+                                dim3(kTreeThreads), smem, st, mk, mv, p))
+    return rc;
   if (p.n_splits == 1) return CBK_OK;
-  cudaLaunchConfig_t cfg = {};
   const int64_t rows = static_cast<int64_t>(a->n_kv_heads) * p.rows;
-  cfg.gridDim = dim3(static_cast<unsigned>((rows + kTreeMergeWarps - 1) / kTreeMergeWarps));
-  cfg.blockDim = dim3(kTreeMergeWarps * 32);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_merge_kernel<DT, HD>, p, static_cast<int>(a->n_kv_heads));
-  if (e != cudaSuccess) return set_error(CBK_ERR_CUDA, "tree_merge_kernel launch: %s", cudaGetErrorString(e));
-  return check_launch("tree_merge_kernel");
+  return launch_dependent("tree_merge_kernel", tree_merge_kernel<DT, HD>,
+                          dim3(static_cast<unsigned>((rows + kTreeMergeWarps - 1) / kTreeMergeWarps)),
+                          dim3(kTreeMergeWarps * 32), 0, st, p, static_cast<int>(a->n_kv_heads));
 }
 
 template <int DT>
