@@ -15,9 +15,11 @@
 // and kNrUnroll passes are a chunk.  Sources arrive by bulk copies into kNrSlots
 // chunks of shared memory per warp, so the bytes in flight cost no registers
 // (loads into registers: 171 us for 32768 tokens of 32 + 8 heads of 128, bound by
-// the loads' latency at the occupancy the registers left; this way 149 us = 5.5 TB/s,
-// 0.84 of measured HBM).  Chunks of 4 passes took 146 us there but 3.8 instead of
-// 3.1 us for one token; 2, 4 or 8 slots, 4 or 8 CTAs of 256 threads were slower.  The sum of squares is
+// the loads' latency at the occupancy the registers left; this way 141 us = 5.8 TB/s,
+// 0.89 of measured HBM).  Chunks of 4 passes were 2 % faster there but took 3.8
+// instead of 3.1 us for one token; 2, 4 or 8 slots, 4 or 8 CTAs of 256 threads were
+// slower, and so was the arithmetic on single floats (158 us: 10 to 20 % more
+// instructions, of which a pass of two heads takes 130).  The sum of squares is
 // a butterfly within the head's lanes.  A warp takes all heads of a token (several
 // warps share one when there are few tokens), so cos, sin and the weights are read
 // and multiplied together once per token: with wc = w c, ws = w s and r the root,
@@ -187,7 +189,7 @@ norm_rope_scatter_kernel(const NormRopeParams p) {
       t0 = __ldg(t);
       t1 = __ldg(t + 1);
     }
-    const bool norm = p.qw != nullptr;
+    const bool norm = p.qw != nullptr, full = p.rotary == p.dim;
     const uint64_t c[2] = {pk_f2(t0.x, t0.z), pk_f2(t1.x, t1.z)}, s[2] = {pk_f2(t0.y, t0.w), pk_f2(t1.y, t1.w)};
     const uint32_t c16[2] = {narrow<DT>(c[0]), narrow<DT>(c[1])}, s16[2] = {narrow<DT>(s[0]), narrow<DT>(s[1])};
 
@@ -261,6 +263,12 @@ norm_rope_scatter_kernel(const NormRopeParams p) {
                 z.a[i] = Pk<DT>::sub(Pk<DT>::mul(y.a[i], c16[i]), Pk<DT>::mul(y.b[i], s16[i]));
                 z.b[i] = Pk<DT>::add(Pk<DT>::mul(y.b[i], c16[i]), Pk<DT>::mul(y.a[i], s16[i]));
               }
+            }
+          } else if (full) {                         // every lane turns: no selects (149 -> 141 us)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              z.a[i] = narrow<DT>(mul_f2(fma_f2(a[i], ca[i], mul_f2(b[i], sb[i])), rr));
+              z.b[i] = narrow<DT>(mul_f2(fma_f2(b[i], cb[i], mul_f2(a[i], sa[i])), rr));
             }
           } else if (turns || norm) {
 #pragma unroll
