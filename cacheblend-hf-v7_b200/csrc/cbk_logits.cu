@@ -14,8 +14,10 @@
 //
 // process_logits_kernel: a cluster of CTAs takes a row (several rows, one after the
 // other, when there are more rows than clusters fit), each CTA every n-th block of
-// 128 tokens of the vocabulary.  A thread takes vectors of 8 logits (16 or 32 bytes),
-// kBatch loads in flight, the first batch before any counting.  The row's choice is a
+// 128 tokens of the vocabulary.  A thread takes one vector of 8 logits (16 or 32 bytes)
+// at a time, with its counts and mask bits loaded beside it, the first one before any
+// counting; 32 warps to an SM hide the latency better than more vectors a thread did (2
+// and 4 vectors: the same and 10 % slower).  The row's choice is a
 // maximum over 64-bit keys (order of x, then lowest index) in the CTA and over the
 // cluster, so no order of atomics shows.  Rows that do not lie on 16-byte boundaries
 // are read element by element, neighbouring lanes on neighbouring elements.
@@ -183,7 +185,7 @@ count_tokens_kernel(const LogitsParams p) {
 template <int IN, int OUT, int VEC>
 __global__ void __launch_bounds__(kLgThreads, 2)
 process_logits_kernel(const LogitsParams p) {
-  constexpr int kBatch = VEC == 1 ? 8 : IN == CBK_F32 ? 2 : 4;
+  constexpr int kBatch = VEC == 1 ? 8 : 1;
   // counts [seg] (when the CTA counts), path bits [seg / 256] and path [n_tree] (with a tree)
   extern __shared__ __align__(16) uint32_t s_dyn[];
   __shared__ int s_n_path;
@@ -292,6 +294,20 @@ process_logits_kernel(const LogitsParams p) {
     const int n_batches = (p.seg + kBatch * kLgThreads * VEC - 1) / (kBatch * kLgThreads * VEC);
     for (int b = 0; b < n_batches; ++b) {
       if (b > 0) load_batch(b);
+      // the vector's counts and mask bits on their way beside it
+      uint4 c_lo = make_uint4(0, 0, 0, 0), c_hi = c_lo;
+      uint32_t bits = 0xffu;
+      if (VEC == 8) {
+        const int o = offset(b, 0), i = token_at(o);
+        if (o < p.seg && i + VEC <= p.vocab) {
+          if (p.counts) {
+            c_lo = *reinterpret_cast<const uint4*>(p.counts + i);
+            c_hi = *reinterpret_cast<const uint4*>(p.counts + i + 4);
+          }
+          // i is a multiple of 8: the 8 bits are one byte of the row
+          if (p.mask) bits = __ldg(reinterpret_cast<const uint8_t*>(p.mask + row * p.mask_stride) + i / 8);
+        }
+      }
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         const int o = offset(b, k), i = token_at(o);
@@ -301,18 +317,13 @@ process_logits_kernel(const LogitsParams p) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) x[e] = raw[k].at(e);
           if (p.history || n_path > 0) {
-            uint32_t n[VEC], any = 0;
-#pragma unroll
-            for (int q = 0; q < VEC / 4; ++q) {
-              uint4 c4 = make_uint4(0, 0, 0, 0);
-              if (p.counts) c4 = *reinterpret_cast<const uint4*>(p.counts + i + 4 * q);
-              else if (p.history) c4 = *reinterpret_cast<const uint4*>(s_count + o + 4 * q);
-              n[4 * q] = c4.x;
-              n[4 * q + 1] = c4.y;
-              n[4 * q + 2] = c4.z;
-              n[4 * q + 3] = c4.w;
-              any |= c4.x | c4.y | c4.z | c4.w;
+            uint4 lo = c_lo, hi = c_hi;
+            if (counts_here) {
+              lo = *reinterpret_cast<const uint4*>(s_count + o);
+              hi = *reinterpret_cast<const uint4*>(s_count + o + 4);
             }
+            uint32_t n[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            uint32_t any = lo.x | lo.y | lo.z | lo.w | hi.x | hi.y | hi.z | hi.w;
             if (on_path(o)) {
               any = 1;
               for (int j = 0; j < n_path; ++j) {
@@ -338,8 +349,6 @@ process_logits_kernel(const LogitsParams p) {
             }
           }
           if (p.mask) {
-            // i is a multiple of 8: the 8 bits are one byte of the row
-            const uint32_t bits = __ldg(reinterpret_cast<const uint8_t*>(p.mask + row * p.mask_stride) + i / 8);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) x[e] = (bits >> e) & 1u ? x[e] : -INFINITY;
           }
