@@ -622,6 +622,63 @@ def test_a_step_of_the_three(ops):
     assert torch.equal(x.cpu(), exp) and torch.equal(tok.cpu(), exp_tok)
 
 
+def test_calls_on_two_streams_at_once(ops):
+    """Calls that overlap on the GPU, each with its own workspace, give what they give alone."""
+    cases = [ta_inputs(16, 6000, 32, 8, 128, BF, "tree", seed=s) for s in (0, 1)]
+    logits = [pl_inputs(40, 20000, 3000, BF, seed=s) for s in (0, 1)]
+    n = torch.tensor([6000], device=DEV)
+
+    def work(i):
+        q, k, v, words, _ = (x.to(DEV) if isinstance(x, torch.Tensor) else x for x in cases[i])
+        x, h = logits[i][0].to(DEV), logits[i][1].to(DEV)
+        torch.cuda.synchronize()
+        return lambda: [(ops.tree_attn(q, k, v, n, words, 32, 8, 128, 0.09),
+                         *ops.process_logits(x, history=h, repetition=1.2, frequency=0.1)) for _ in range(10)]
+
+    calls = [work(0), work(1)]
+    alone = [c()[0] for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    out = []
+    for c, st in zip(calls, streams):
+        with torch.cuda.stream(st):
+            out.append(c())
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for got in out[i]:
+            for a, b in zip(got, alone[i]):
+                assert torch.equal(a, b)
+
+
+def test_two_captured_graphs_interleaved(ops):
+    """Each captured call keeps its own workspace; lengths that advance on the device are followed."""
+    x, h, _ = pl_inputs(30, 5000, 400, BF)
+    dx, dh, n = x.to(DEV), h.to(DEV), torch.tensor([0], device=DEV)
+    y, h2, _ = pl_inputs(3, 5000, 400, BF, seed=5)
+    dy = y.to(DEV)
+
+    def capture(f):
+        f()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            out = f()
+        torch.cuda.current_stream().wait_stream(side)
+        return graph, out
+
+    kw = dict(repetition=1.3, presence=0.1, frequency=0.2)
+    g1, o1 = capture(lambda: ops.process_logits(dx, history=dh, lengths=n, **kw))
+    g2, o2 = capture(lambda: ops.process_logits(dy, history=dh, lengths=n, **kw))
+    for length in (0, 1, 57, 400):
+        n.fill_(length)
+        g1.replay()
+        g2.replay()
+        for (got, tok), z in ((o1, x), (o2, y)):
+            exp, exp_tok = ref.logits(z, history=h, lengths=torch.tensor([length]), **kw)
+            assert torch.equal(got.cpu(), exp.to(BF)) and torch.equal(tok.cpu(), exp_tok)
+
+
 def test_the_three_repeat_bit_for_bit(ops):
     q, k, v, words, cap = ta_inputs(20, 3000, 32, 8, 128, BF, "tree")
     args = [x.to(DEV) for x in (q, k, v)] + [torch.tensor([3000], device=DEV), words.to(DEV), 32, 8, 128, 0.09]
