@@ -637,8 +637,8 @@ def _tree_workspace_bytes(n_nodes: int, cap: int, n_q_heads: int, n_kv_heads: in
 
 
 def tree_workspace(n_nodes: int, cap: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
-    """Workspace of tree_attn for up to n_nodes nodes over a cache of cap rows
-    (reusable by calls that do not overlap on the GPU)."""
+    """Workspace of tree_attn for n_nodes nodes over a cache of cap rows (reusable by
+    calls that do not overlap on the GPU; another number of nodes may need more)."""
     device = torch.device(device)
     index = torch.cuda.current_device() if device.index is None else device.index
     nbytes = _tree_workspace_bytes(n_nodes, cap, n_q_heads, n_kv_heads, head_dim, index)
