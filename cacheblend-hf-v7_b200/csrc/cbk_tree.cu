@@ -16,9 +16,10 @@
 // TMEM and a softmax warpgroup of its own, so one slot's softmax runs while the
 // tensor core works for the other.  With two Q tiles, slot t is tile t and every
 // key tile goes to both; with one Q tile both slots hold that tile and take the
-// key tiles in turn, each with its own running max, sum and O, joined at the end.  Unit u of a CTA (slot u & 1) is then key tile u >> 1 or
-// u, and the MMA warp's order is the same for both: O += P(u) V(u), then
-// S(u + 2) = Q K(u + 2)^T, which overwrites P(u) after the PV that reads it.
+// key tiles in turn, each with its own running max, sum and O, joined at the end.
+// Unit u of a CTA (slot u & 1) is then key tile u >> 1 or u, and the MMA warp's order
+// is the same for both: O += P(u) V(u), then S(u + 2) = Q K(u + 2)^T, which overwrites
+// P(u) after the PV that reads it.
 //
 // Warps (384 threads): 0 copies K and V tiles (TMA) into two rings; 1 issues the
 // MMAs; 2 holds TMEM; 2 and 3 clean the V tiles that reach past the context; 4..7
@@ -34,6 +35,14 @@
 // Rounding: S, the softmax statistics, O, the partial results and the merge are
 // fp32; P is rounded to the inputs' 16-bit type for the PV MMA (the tensor core
 // takes both operands in one type), the result once.
+//
+// Measured, 32 q heads on 8 KV heads of 128, bf16, both kernels of the call: 24 nodes over
+// 131072 keys 92 us (537 MB: 5.85 TB/s, 0.90 of measured HBM; 99 us in a long loop), 1
+// node 86 us (6.2 TB/s);
+// 64 nodes (two Q tiles) over 32768 keys 43 us (790 TFLOP/s with both products counted: a
+// key tile takes both slots 1.9 us, of which the exponentials alone 1.3); 16 nodes over
+// 6208 keys 13.5 us, 1 node 10.5 (HBM alone 3.9: set-up 1.5, key tiles 3.3, epilogue 1,
+// merge launch and merge 3.5).
 // Every wait is bounded; on timeout the kernel sets CBK_STATUS_TIMEOUT, drains its
 // copies and MMAs, frees TMEM and returns.
 #include <algorithm>
@@ -101,25 +110,33 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
-template <int HD, int NQ, int NST>
+template <int HD, int NQ>
 struct TreeSmem {
+  // K and V tiles in flight.  One Q tile, heads of 128: 3 against 2 is 17.1 against 17.7
+  // us for 8 nodes over 12000 keys, 93 against 100 for 24 over 131072 in a long loop (in
+  // a short one 91.3 against 90.5) and 13.4 against 12.6 for 16 over 6208; heads of 64:
+  // 3 against 6 is 16.9 against 18.0 for 7 nodes over 32768, 40.8 against 41.6 for 24
+  // over 131072.  Two Q tiles: 3 do not fit with heads of 128; heads of 64, 64 nodes
+  // over 16384: 18.9 with 2, 19.1 with 3 or 5.
+  static constexpr int kStages = NQ == 1 ? 3 : 2;
   static constexpr int kQBytes = kBM * HD * 2;
   static constexpr int kKVBytes = kBN * HD * 2;
   static constexpr int kK0 = NQ * kQBytes;
-  static constexpr int kV0 = kK0 + NST * kKVBytes;
-  static constexpr int kBar = kV0 + NST * kKVBytes;
-  static constexpr int kBars = 5 * NST + 9;
+  static constexpr int kV0 = kK0 + kStages * kKVBytes;
+  static constexpr int kBar = kV0 + kStages * kKVBytes;
+  static constexpr int kBars = 5 * kStages + 9;
   static constexpr int kMisc = kBar + kBars * 8;       // tmem slot, abort flag, non-finite flag
   static constexpr int kTotal = kMisc + 16;
   // more than half an SM's shared memory: one CTA (holding all 512 TMEM columns) per SM
   static constexpr int kAlloc = (kTotal + 1024) > 122880 ? (kTotal + 1024) : 122880;
 };
 
-template <int DT, int HD, int NQ, int NST>
+template <int DT, int HD, int NQ>
 __global__ void __launch_bounds__(kTreeThreads, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                  const TreeParams p) {
-  using L = TreeSmem<HD, NQ, NST>;
+  using L = TreeSmem<HD, NQ>;
+  constexpr int NST = L::kStages;
   enum { KFULL = 0, KEMPTY = NST, VFULL = 2 * NST, VEMPTY = 3 * NST, VCLEAN = 4 * NST, SFULL = 5 * NST,
          PHALF = SFULL + 2, PFULL = SFULL + 4, ODONE = SFULL + 6, DRAIN = SFULL + 8 };
   const int split = blockIdx.x, kvh = blockIdx.y, pair = blockIdx.z;
@@ -544,7 +561,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 
 // Merge of the splits, a warp per query row: O = sum_i w_i O_i / sum_i w_i l_i,
 // w_i = 2^(m_i - M) over the splits that hold a key tile, in their order, sixteen O
-// loads in flight.  A row that sees nothing has every l_i = 0 and gets zeros.
+// loads in flight (behind branches, one by one: 24 us instead of 10 for 64 nodes over
+// 32768 keys, 19 MB of partial results).  A row that sees nothing has every l_i = 0 and
+// gets zeros.
 // (With one such split the attention kernel has written the output.)
 template <int DT, int HD>
 __global__ void __launch_bounds__(kTreeMergeWarps * 32)
@@ -643,13 +662,13 @@ static TreeLayout tree_layout(int n_nodes, int64_t cap, int n_q_heads, int n_kv_
   return t;
 }
 
-template <int DT, int HD, int NQ, int NST>
+template <int DT, int HD, int NQ>
 static int launch_tree(const cbk_tree_attn_args* a, const TreeParams& p, cudaStream_t st) {
   CUtensorMap mk, mv;
   if (int rc = attn_make_map(&mk, a->k_cache, DT, HD, a->n_kv_heads, a->cap, a->kv_row_stride, 1, kBN)) return rc;
   if (int rc = attn_make_map(&mv, a->v_cache, DT, HD, a->n_kv_heads, a->cap, a->kv_row_stride, 1, kBN)) return rc;
-  auto kern = tree_attn_kernel<DT, HD, NQ, NST>;
-  constexpr int smem = TreeSmem<HD, NQ, NST>::kAlloc;
+  auto kern = tree_attn_kernel<DT, HD, NQ>;
+  constexpr int smem = TreeSmem<HD, NQ>::kAlloc;
   static_assert(smem <= 227 * 1024, "shared memory of tree_attn_kernel");
   if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), smem)) return rc;
   if (int rc = launch_dependent("tree_attn_kernel", kern, dim3(p.n_splits, a->n_kv_heads, p.n_pairs),
@@ -664,11 +683,11 @@ static int launch_tree(const cbk_tree_attn_args* a, const TreeParams& p, cudaStr
 
 template <int DT>
 static int dispatch_tree(const cbk_tree_attn_args* a, const TreeParams& p, cudaStream_t st) {
-  // one Q tile: a deeper ring (the call is bound by reading K and V); two: their
-  // second tile takes a stage's room
-  if (a->head_dim == 128)
-    return p.n_qt == 1 ? launch_tree<DT, 128, 1, 3>(a, p, st) : launch_tree<DT, 128, 2, 2>(a, p, st);
-  return p.n_qt == 1 ? launch_tree<DT, 64, 1, 6>(a, p, st) : launch_tree<DT, 64, 2, 5>(a, p, st);
+  // One Q tile in both slots or two: the first could run as the second with one tile,
+  // but takes less room and is faster alone (7 nodes of 7 heads of 64 over 32768 keys
+  // 16.9 us against 17.4, 37 nodes over 1029 7.2 against 7.4).
+  if (a->head_dim == 128) return p.n_qt == 1 ? launch_tree<DT, 128, 1>(a, p, st) : launch_tree<DT, 128, 2>(a, p, st);
+  return p.n_qt == 1 ? launch_tree<DT, 64, 1>(a, p, st) : launch_tree<DT, 64, 2>(a, p, st);
 }
 
 }  // namespace cbk
