@@ -21,7 +21,11 @@
 // keys (order of x, then lowest index) in the CTA and over the cluster, so no order of
 // atomics shows.  Rows that do not lie on 16-byte boundaries are read element by
 // element, neighbouring lanes on neighbouring elements.  64 rows of 128256 after 24 K
-// tokens: 29 us, bound by instructions and latency (its bytes would take 5.3).
+// tokens: 26 us, bound by instructions and latency (its bytes would take 5.3); 16 rows
+// after 5 K 14, one row of 32000 after 6 K 5.9.
+//
+// Penalties come element by element, each behind a branch, or, with a history long for
+// its vocabulary (DENSE), for a whole vector in packed pairs without branches.
 //
 // Counts per token (bits 0-30 made, bit 31 in the prompt) come about in one of two
 // ways.  Few rows, or a history per row: a CTA reads the whole history and counts what
@@ -31,7 +35,7 @@
 // adds is a short list per row; a bit per vector of 8 tokens says where to look it up.
 #include <algorithm>
 
-#include "cbk_common.cuh"
+#include "cbk_attn_common.cuh"
 
 namespace cbk {
 
@@ -47,6 +51,11 @@ constexpr int kLgCountCtas = 8;                         // CTAs that count a sha
 // tokens: 29.6 us against 52.9 with every cluster counting; 16 rows after 5 K: 14.5
 // against 14.1), and clusters that fit side by side, two CTAs to an SM.
 constexpr int kLgManyRows = 24, kLgFit8 = 30, kLgFit4 = 66;
+// A history's room over the vocabulary from which a vector's penalties are computed in
+// pairs, seen or not, instead of each behind a branch (64 rows of 128256: a history of
+// 24 K tokens 25.3 us with branches, 23.2 without, 12 K 23.3 and 22.7, 6 K 21.1 and 22.4,
+// 3 K 19.5 and 21.9; one row of 32000 after 6 K 6.6 and 6.0).
+constexpr int kLgDense = 16;
 constexpr uint32_t kLgPrompt = 0x80000000u;
 
 struct LogitsParams {
@@ -61,7 +70,7 @@ struct LogitsParams {
   int64_t row_stride, out_stride, hist_stride, hist_cap, len_stride, prompt_stride, bias_stride, mask_stride,
       tree_stride;
   int rows, vocab, seg, n_tree, shared, log_cluster;
-  float repetition, inv_repetition, presence, frequency;
+  float repetition, inv_repetition, inv_rest, presence, frequency;   // inv_rest: what 1 / repetition has beyond 24 bits
 };
 
 // order of fp32 values as unsigned integers: -inf < ... < -0 = +0 < ... < inf < NaN
@@ -108,6 +117,27 @@ __device__ __forceinline__ float divide(float x, float b, float y) {
   float q = __fmul_rn(x, y);
   q = __fmaf_rn(__fmaf_rn(-q, b, x), y, q);
   return __fmaf_rn(__fmaf_rn(-q, b, x), y, q);
+}
+
+// one seen element's penalties
+__device__ __forceinline__ float penalise1(float x, uint32_t n, float rep, float inv, float freq, float pres) {
+  x = x > 0.f ? divide(x, rep, inv) : __fmul_rn(x, rep);
+  const uint32_t c = n & ~kLgPrompt;
+  return c ? __fsub_rn(__fsub_rn(x, __fmul_rn(freq, static_cast<float>(c))), pres) : x;
+}
+// (as a call, where it is the rare case and would only fill the instruction cache)
+__device__ __noinline__ float penalise_apart(float x, uint32_t n, float rep, float inv, float freq, float pres) {
+  return penalise1(x, n, rep, inv, freq, pres);
+}
+
+// whether the magnitudes of 8 numbers are in divide's range
+__device__ __forceinline__ bool in_range(const float* x) {
+  const float hi = max3f(max3f(fabsf(x[0]), fabsf(x[1]), fabsf(x[2])), max3f(fabsf(x[3]), fabsf(x[4]), fabsf(x[5])),
+                         fmaxf(fabsf(x[6]), fabsf(x[7])));
+  float lo = fminf(fabsf(x[0]), fabsf(x[1]));
+#pragma unroll
+  for (int e = 2; e < 8; ++e) lo = fminf(lo, fabsf(x[e]));
+  return lo > 1e-20f && hi < 1e20f;
 }
 
 // max that propagates NaN
@@ -184,7 +214,7 @@ count_tokens_kernel(const LogitsParams p) {
   grid_launch_dependents();
 }
 
-template <int IN, int OUT, int VEC>
+template <int IN, int OUT, int VEC, bool DENSE>
 __global__ void __launch_bounds__(kLgThreads, 2)
 process_logits_kernel(const LogitsParams p) {
   constexpr int kBatch = VEC == 1 ? 8 : 1;
@@ -274,12 +304,36 @@ process_logits_kernel(const LogitsParams p) {
     float best = -INFINITY;
     int best_i = token_at(tid * VEC);                     // the thread's first element: the first of a row of -inf
     auto penalise = [&](float x, uint32_t n) {
-      if (n) {
-        x = x > 0.f ? divide(x, p.repetition, p.inv_repetition) : __fmul_rn(x, p.repetition);
-        const uint32_t c = n & ~kLgPrompt;
-        if (c) x = __fsub_rn(__fsub_rn(x, __fmul_rn(p.frequency, static_cast<float>(c))), p.presence);
+      if (!n) return x;
+      if constexpr (DENSE) return penalise_apart(x, n, p.repetition, p.inv_repetition, p.frequency, p.presence);
+      else return penalise1(x, n, p.repetition, p.inv_repetition, p.frequency, p.presence);
+    };
+    // the same for a vector, in pairs and without branches.  With y + y_rest = 1 / rep to
+    // twice the bits the first q is within one unit of the quotient, and divide's last
+    // step makes it the rounded one.
+    auto penalise8 = [&](float* x, const uint32_t* n) {
+      const uint64_t y = pk_f2(p.inv_repetition, p.inv_repetition), y_rest = pk_f2(p.inv_rest, p.inv_rest);
+      const uint64_t rep = pk_f2(p.repetition, p.repetition), neg_rep = pk_f2(-p.repetition, -p.repetition);
+      const uint64_t neg_magic = pk_f2(-8388608.f, -8388608.f);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const uint64_t v = pk_f2(x[e], x[e + 1]);
+        uint64_t q = fma_f2(v, y, mul_f2(v, y_rest));
+        q = fma_f2(fma_f2(q, neg_rep, v), y, q);
+        float a[2], b[2];
+        upk_f2(q, a[0], a[1]);
+        upk_f2(mul_f2(v, rep), b[0], b[1]);
+        uint64_t z = pk_f2(x[e] > 0.f ? a[0] : b[0], x[e + 1] > 0.f ? a[1] : b[1]);
+        // c < 2^23 as a float: 2^23 + c has c's bits in its mantissa
+        const uint32_t c0 = n[e] & ~kLgPrompt, c1 = n[e + 1] & ~kLgPrompt;
+        upk_f2(add_f2(pk_f2(__uint_as_float(c0 | 0x4b000000u), __uint_as_float(c1 | 0x4b000000u)), neg_magic), b[0], b[1]);
+        // (a packed product would be contracted with the sum, which then rounds once)
+        z = add_f2(z, pk_f2(__fmul_rn(-p.frequency, b[0]), __fmul_rn(-p.frequency, b[1])));
+        z = add_f2(z, pk_f2(c0 ? -p.presence : 0.f, c1 ? -p.presence : 0.f));
+        upk_f2(z, a[0], a[1]);
+        x[e] = n[e] ? a[0] : x[e];
+        x[e + 1] = n[e + 1] ? a[1] : x[e + 1];
       }
-      return x;
     };
     auto take = [&](float x, int i) {
       if (x > best || (x != x && best == best)) {
@@ -288,6 +342,8 @@ process_logits_kernel(const LogitsParams p) {
       }
     };
     const int n_path = p.n_tree > 0 ? s_n_path : 0;
+    const bool paired = DENSE && p.inv_repetition != 0.f && fabsf(p.presence) < INFINITY &&
+                        fabsf(p.frequency) < INFINITY;
     auto on_path = [&](int o) { return n_path > 0 && ((s_over[o / 256] >> (o / 8 % 32)) & 1u); };
     const int n_batches = (p.seg + kBatch * kLgThreads * VEC - 1) / (kBatch * kLgThreads * VEC);
     for (int b = 0; b < n_batches; ++b) {
@@ -352,8 +408,11 @@ process_logits_kernel(const LogitsParams p) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) n[e] += at == e ? 1u : 0u;
               }
+              if (DENSE) any = n[0] | n[1] | n[2] | n[3] | n[4] | n[5] | n[6] | n[7];
             }
-            if (any) {
+            if (paired && any && (any & ~kLgPrompt) < (1u << 23) && in_range(x)) {
+              penalise8(x, n);
+            } else if (any) {
 #pragma unroll
               for (int e = 0; e < VEC; ++e) x[e] = penalise(x[e], n[e]);
             }
@@ -450,9 +509,9 @@ process_logits_kernel(const LogitsParams p) {
   }
 }
 
-template <int IN, int OUT, int VEC>
+template <int IN, int OUT, int VEC, bool DENSE>
 static int launch_logits(const LogitsParams& p, cudaStream_t st) {
-  auto kern = process_logits_kernel<IN, OUT, VEC>;
+  auto kern = process_logits_kernel<IN, OUT, VEC, DENSE>;
   const int smem = ((p.history && !p.counts ? p.seg : 0) + (p.n_tree > 0 ? (p.seg + 255) / 256 + p.n_tree : 0)) * 4;
   if (int rc = ensure_smem_attr(reinterpret_cast<const void*>(kern), kLgMaxSmem)) return rc;
   if (p.log_cluster > 3) {
@@ -573,6 +632,8 @@ extern "C" int cbk_process_logits(const cbk_process_logits_args* a, void* stream
   p.repetition = a->repetition;
   p.inv_repetition = a->repetition >= 0x1p-40f && a->repetition <= 0x1p40f
       ? static_cast<float>(1.0 / static_cast<double>(a->repetition)) : 0.f;
+  p.inv_rest = p.inv_repetition == 0.f ? 0.f
+      : static_cast<float>(1.0 / static_cast<double>(a->repetition) - static_cast<double>(p.inv_repetition));
   p.presence = a->presence;
   p.frequency = a->frequency;
   auto st = static_cast<cudaStream_t>(stream);
@@ -582,8 +643,10 @@ extern "C" int cbk_process_logits(const cbk_process_logits_args* a, void* stream
   const uint64_t off = reinterpret_cast<uintptr_t>(a->logits) | (a->rows > 1 ? a->row_stride * in_size : 0) |
                        (a->out ? reinterpret_cast<uintptr_t>(a->out) | (a->rows > 1 ? a->out_stride * out_size : 0) : 0) |
                        (a->bias ? reinterpret_cast<uintptr_t>(a->bias) | (a->bias_stride * 4) : 0);
-  const bool vec = (off & 15u) == 0;
-#define CBK_LG(IN, OUT) return vec ? launch_logits<IN, OUT, 8>(p, st) : launch_logits<IN, OUT, 1>(p, st)
+  const bool vec = (off & 15u) == 0, dense = p.history && a->history_cap * kLgDense >= a->vocab;
+#define CBK_LG(IN, OUT)                                                             \
+  return !vec ? launch_logits<IN, OUT, 1, false>(p, st)                             \
+              : dense ? launch_logits<IN, OUT, 8, true>(p, st) : launch_logits<IN, OUT, 8, false>(p, st)
   switch (a->in_dtype) {
     case CBK_F32: CBK_LG(CBK_F32, CBK_F32);
     case CBK_BF16:

@@ -56,11 +56,6 @@ struct NormRopeParams {
   float eps, inv_dim;
 };
 
-__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // a packed 16-bit pair as an fp32 pair
 template <int DT>
 __device__ __forceinline__ uint64_t widen(uint32_t w) {

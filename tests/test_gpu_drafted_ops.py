@@ -440,6 +440,35 @@ def test_process_logits(ops, rows, vocab, length, dt, out, shared):
     pl_check(ops, x, out)
 
 
+@pytest.mark.parametrize("dt,out", [(BF, None), (BF, torch.float32), (HF, None), (torch.float32, None)])
+@pytest.mark.parametrize("rows,vocab", [(1, 32000), (3, 4104), (30, 4096)])
+def test_process_logits_long_history(ops, rows, vocab, dt, out):
+    """A history long for its vocabulary: magnitudes from 0 to infinity among seen
+    and unseen tokens, every penalty's extremes, a path on top; and the same rows
+    with their tokens at the front of a history with much more or no more room."""
+    x, h, g = pl_inputs(rows, vocab, 4000, dt, seed=7)
+    odd = torch.tensor([0.0, -0.0, 1e-45, 1e-40, 1e-30, 9e-21, 1.1e-20, 1e20, 3e38, -1e-30, -3e38, float("inf"),
+                        -float("inf"), float("nan")])
+    at = torch.randperm(vocab - 8, generator=g)[:4 * len(odd)].view(4, -1)
+    x[:, at[0]] = odd.to(dt)
+    x[:, at[1]] = odd.to(dt)
+    h[0, 100:100 + len(odd)] = at[0]                  # at[1] unseen but for chance
+    words, _ = ops.tree_words([-1] + [i // 2 for i in range(rows - 1)])
+    toks = torch.cat([at[2], at[0], h[0, :8]])[:rows]
+    for kw in (dict(repetition=1.1, presence=0.25, frequency=0.125), dict(repetition=0.3, presence=-2.0, frequency=-0.7),
+               dict(repetition=3.0), dict(frequency=0.3), dict(presence=0.7), dict(repetition=2.0 ** 41, presence=1.0),
+               dict(repetition=1e-30), dict(repetition=1.2, frequency=float("inf")),
+               dict(repetition=1.2, presence=-float("inf"))):
+        assert pl_check(ops, x, out, history=h, n_prompt=torch.tensor([1500]), **kw) == 0
+        assert pl_check(ops, x, out, history=h, n_prompt=torch.tensor([3990]), tree_tokens=toks, tree_words=words,
+                        **kw) == 0
+    kw = dict(repetition=1.1, presence=0.25, frequency=0.125, out_dtype=out)
+    few = h[:, :vocab // 16 - 1].contiguous().to(DEV)
+    a, t = ops.process_logits(x.to(DEV), history=h.to(DEV), lengths=torch.tensor([few.shape[1]], device=DEV), **kw)
+    b, u = ops.process_logits(x.to(DEV), history=few, **kw)
+    assert torch.equal(a.nan_to_num(0.5), b.nan_to_num(0.5)) and torch.equal(t, u)
+
+
 @pytest.mark.parametrize("dt", [BF, HF, torch.float32])
 def test_process_logits_every_alignment(ops, dt):
     """Rows of a wider buffer from every first element, and odd output strides."""
