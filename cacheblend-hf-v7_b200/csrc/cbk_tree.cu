@@ -111,6 +111,16 @@ __device__ __forceinline__ uint32_t tree_bits(const uint32_t* w, int n, int off)
   return __funnelshift_r(word(off >> 5), word((off >> 5) + 1), off & 31);
 }
 
+// 1 / l of a row; without any weight 0, or NaN (the formula's 0 / 0) when the row sees
+// keys after all, each with a score of -inf
+__device__ __forceinline__ float tree_inverse(const TreeParams& p, int64_t n_ctx, int node, float l) {
+  if (l != 0.f) return 1.f / l;
+  bool sees = n_ctx > 0;
+  for (int off = 0; off < p.n_nodes && !sees; off += 32)
+    sees = tree_bits(p.words + node * p.words_stride, p.n_nodes, off) != 0;
+  return sees ? __int_as_float(0x7fffffff) : 0.f;
+}
+
 // 16 bytes from global to shared memory, asynchronously; zeros when not `there`
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -499,7 +509,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         float* po = p.part_o + (slot * p.row_pitch + row) * HD;
         const int grow = (2 * pair + (two ? t : 0)) * kBM + row;
         uint16_t* out = p.out + (static_cast<int64_t>(node) * p.n_q + kvh * p.group + grow % p.group) * HD;
-        const float inv = l_sum == 0.f ? 0.f : 1.f / l_sum;
+        const float inv = direct ? tree_inverse(p, sp.n_ctx, node, l_sum) : 1.f;
         const bool fix = *odd_flag != 0;
         const uint32_t t_other = tmem + 256 * (t ^ 1) + lane_off + kBN;
         // columns of 32: this warp's share
@@ -567,8 +577,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 // Merge of the splits, a warp per query row: O = sum_i w_i O_i / sum_i w_i l_i,
 // w_i = 2^(m_i - M) over the splits that hold a key tile, in their order, sixteen O
 // loads in flight (behind branches, one by one: 24 us instead of 10 for 64 nodes over
-// 32768 keys, 19 MB of partial results).  A row that sees nothing has every l_i = 0 and
-// gets zeros.
+// 32768 keys, 19 MB of partial results).  A row that sees nothing has every l_i = 0.
 // (With one such split the attention kernel has written the output.)
 template <int DT, int HD>
 __global__ void __launch_bounds__(kTreeMergeWarps * 32)
@@ -637,7 +646,7 @@ tree_merge_kernel(const TreeParams p, int n_kv) {
       }
     }
   }
-  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+  const float inv = tree_inverse(p, sp.n_ctx, row / p.group, lsum);
   uint16_t* o = p.out + (static_cast<int64_t>(row / p.group) * p.n_q + kvh * p.group + row % p.group) * HD + lane * kD;
 #pragma unroll
   for (int d = 0; d < kD; d += 2) *reinterpret_cast<uint32_t*>(o + d) = Pk<DT>::cvt(acc[d] * inv, acc[d + 1] * inv);

@@ -62,3 +62,32 @@ def test_tree_attn_nonfinite_context_keys(ops, t, n_ctx, hq, hkv, d, dt):
         assert ok.any() and not ok.all()
         bound = ref.tree_bound(out, A, n, dt, huge)
         assert ((got.double() - out).abs() <= bound)[ok].all(), col
+
+
+@pytest.mark.parametrize("t,n_ctx,hq,hkv,d,dt", [
+    (6, 0, 8, 2, 64, BF), (6, 3, 8, 2, 128, HF),      # one key tile: the attention kernel writes the output
+    (6, 300, 8, 2, 128, BF),                          # several splits, merged
+    (6, 900, 76, 76, 64, BF),                         # one CTA for all tiles, both slots joined
+    (50, 300, 8, 2, 64, HF),                          # two Q tiles
+])
+def test_tree_attn_rows_of_infinitely_low_scores(ops, t, n_ctx, hq, hkv, d, dt):
+    """A row that sees keys, all with a score of -inf, is 0 / 0 as in the formula; one
+    that sees nothing is 0; one finite score among them has all the weight."""
+    g = torch.Generator().manual_seed(t + n_ctx)
+    cap = n_ctx + t + 5
+    q = (torch.rand((t, hq * d), generator=g) + 0.5).to(dt)
+    k = torch.full((cap, hkv * d), -float("inf"), dtype=dt)
+    v = torch.randn((cap, hkv * d), generator=g).to(dt)
+    k[n_ctx + 2] = 0.25                                # node 2's own key
+    words = torch.zeros((t, (t + 31) // 32), dtype=torch.int32)
+    words[0, 0], words[2, 0], words[3, 0], words[5, 0] = 1, 4, 0b1110, -1 << (t % 32) if t < 32 else 0
+    got = ops.tree_attn(q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor([n_ctx], device=DEV), words.to(DEV), hq, hkv, d,
+                        0.1).cpu()
+    low = torch.full((t,), n_ctx > 0)                  # the context alone
+    low[0], low[2], low[3] = True, False, False
+    assert torch.isnan(got[low]).all()
+    one = v[n_ctx + 2].view(hkv, 1, d).expand(hkv, hq // hkv, d).reshape(-1)
+    assert torch.equal(got[2], one) and torch.equal(got[3], one)
+    rest = ~low
+    rest[2:4] = False
+    assert (got[rest] == 0).all()                      # (bits behind the tree are no rows)
