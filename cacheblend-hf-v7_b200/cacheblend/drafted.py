@@ -100,7 +100,7 @@ class _TreeState:
         self.dev.copy_(h, non_blocking=True)
 
 
-def _tree_step(lw, pre, st: _TreeState, choice: _Choice, status) -> None:
+def _tree_step(lw, pre, st: _TreeState, choice: _Choice, rope_mode: str, status) -> None:
     """The decoder over the nodes in st: their K/V into their cache rows, the token
     after each of them into st.chosen -- all on the device."""
     inner, geo = lw._inner, pre.geo
@@ -112,7 +112,7 @@ def _tree_step(lw, pre, st: _TreeState, choice: _Choice, status) -> None:
         hn = _norm(layer.input_layernorm, h, delta=m, sum_out=h if m is not None else None, status=status)
         q, k, v = _qkv(attn, hn, w_qkv)
         q_rot = ops.norm_rope_scatter(q[0], k[0], v[0], st.pos, st.rows, geo.n_q, geo.n_kv, geo.head_dim, pre.rope,
-                                      pre.fused_k[li], pre.fused_v[li], status=status)
+                                      pre.fused_k[li], pre.fused_v[li], mode=rope_mode, status=status)
         a = ops.tree_attn(q_rot, pre.fused_k[li], pre.fused_v[li], st.n_ctx, st.words, geo.n_q, geo.n_kv, geo.head_dim,
                           geo.scaling, workspace=st.ws, status=status)
         o = attn.o_proj(a.unsqueeze(0))
@@ -189,9 +189,9 @@ def generate_drafted(layerwise_model, chunks: list[Chunk], kv_store: KVStore, ma
             if graph is not None:
                 graph.replay()
             else:
-                _tree_step(lw, pre, st, choice, status)     # eager: first use sets up every kernel
+                _tree_step(lw, pre, st, choice, rope_mode, status)   # eager: first use sets up every kernel
                 if use_graph and len(out) + 1 < max_new_tokens:
-                    graph = _capture(lw, pre, st, choice, status)
+                    graph = _capture(lw, pre, st, choice, rope_mode, status)
                     graph.replay()                                     # (the same nodes again: the same result)
             chosen = st.chosen.tolist()
             path = _accept(tokens, parents, chosen)
@@ -211,14 +211,14 @@ def generate_drafted(layerwise_model, chunks: list[Chunk], kv_store: KVStore, ma
     return (*result, steps) if return_logits else (result, steps)
 
 
-def _capture(lw, pre, st, choice, status):
+def _capture(lw, pre, st, choice, rope_mode, status):
     cur = torch.cuda.current_stream(lw.device)
     side = torch.cuda.Stream(device=lw.device)
     side.wait_stream(cur)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.stream(side):
         with torch.cuda.graph(graph, stream=side):
-            _tree_step(lw, pre, st, choice, status)
+            _tree_step(lw, pre, st, choice, rope_mode, status)
     cur.wait_stream(side)
     return graph
 

@@ -134,7 +134,7 @@ def _mlp1(layer, hn, w_gu):
     return ops.gemv(down.weight, ops.silu_mul(gu[..., :inter], gu[..., inter:]))
 
 
-def _decode_step(lw, pre, st: _DecodeState, status):
+def _decode_step(lw, pre, st: _DecodeState, rope_mode: str, status):
     """One token at position st.pos: its K/V into cache row pos, the next token
     into st.token / st.tokens, pos advanced -- all on the device, no host sync
     (so the step can be captured in a CUDA graph)."""
@@ -148,7 +148,7 @@ def _decode_step(lw, pre, st: _DecodeState, status):
         hn = _norm(layer.input_layernorm, h, delta=m, sum_out=h if m is not None else None, status=status)
         q, k, v = _qkv1(attn, hn, w_qkv)
         q_rot = ops.rope_scatter(q[0], k[0], v[0], st.pos, False, cap, geo.n_q, geo.n_kv, geo.head_dim, pre.rope,
-                                 pre.fused_k[li], pre.fused_v[li], status=status)
+                                 pre.fused_k[li], pre.fused_v[li], mode=rope_mode, status=status)
         # the whole capacity with the position as the causal bound: rows past pos are
         # invisible (and zero), so the call does not change from step to step
         if st.one_row:
@@ -226,7 +226,7 @@ def generate_greedy(layerwise_model, chunks: list[Chunk], kv_store: KVStore, max
             st = _DecodeState(lw, pre, max_new_tokens, pre.logits[0, -1], return_logits, choice)
             n_steps = max_new_tokens - 1
             if n_steps >= 1:
-                _decode_step(lw, pre, st, status)          # eager: first use sets up every kernel
+                _decode_step(lw, pre, st, rope_mode, status)   # eager: first use sets up every kernel
             if n_steps >= 2:
                 if use_graph:
                     cur = torch.cuda.current_stream(lw.device)
@@ -235,7 +235,7 @@ def generate_greedy(layerwise_model, chunks: list[Chunk], kv_store: KVStore, max
                     graph = torch.cuda.CUDAGraph()
                     with torch.cuda.stream(side):
                         with torch.cuda.graph(graph, stream=side):
-                            _decode_step(lw, pre, st, status)
+                            _decode_step(lw, pre, st, rope_mode, status)
                     cur.wait_stream(side)
                     # capture recorded the step without running it
                     for _ in range(n_steps - 1):
@@ -243,7 +243,7 @@ def generate_greedy(layerwise_model, chunks: list[Chunk], kv_store: KVStore, max
                     del graph
                 else:
                     for _ in range(n_steps - 1):
-                        _decode_step(lw, pre, st, status)
+                        _decode_step(lw, pre, st, rope_mode, status)
             tokens = st.tokens.tolist()
             if eos_token_id is not None and eos_token_id in tokens:
                 tokens = tokens[:tokens.index(eos_token_id) + 1]

@@ -1,0 +1,42 @@
+"""Decode over the blended cache at its edges: how keys are rotated, a model
+without a vocabulary size in its configuration, ends inside an accepted path, and
+how many steps run."""
+import pytest
+import torch
+
+import drafted_ref as ref
+from test_gpu_fusor import _setup
+from test_gpu_generate_drafted import CFG128, oracle_draft
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("drafted", [False, True])
+def test_decode_rotates_in_the_mode_asked_for(drafted, monkeypatch):
+    """rope_mode "fp32": the K row of every decoded token is within one rounding of
+    the rotation, as the prompt's are ("ref" rounds cos, sin and each product)."""
+    cb, lw, model, chunks, store = _setup(CFG128, n_chunks=4, chunk_len=100, q_len=20, seed=4)
+    name = "norm_rope_scatter" if drafted else "rope_scatter"
+    plain, rows_seen = getattr(cb.ops, name), []
+
+    def spy(q, k, v, pos, *args, **kw):
+        out = plain(q, k, v, pos, *args, **kw)
+        if q.shape[0] <= 8:                                   # a decode step, not the prefill
+            if drafted:
+                rows, hq, hkv, d, rope, kc, _ = args
+            else:
+                rows, (_, _, hq, hkv, d, rope, kc, _) = pos, args
+            on = rows >= 0
+            z, mag = ref.norm_rope(k[on], hkv, d, None, 0.0, rope, pos[on], False)
+            bound = ref.norm_rope_bound(z, mag, k.dtype, "fp32")
+            rows_seen.append(bool(((kc[rows[on]].double() - z).abs() <= bound).all()))
+        return out
+
+    monkeypatch.setattr(cb.ops, name, spy)
+    run = cb.generate_drafted if drafted else cb.generate_greedy
+    kw = dict(max_nodes=8) if drafted else {}
+    run(lw, chunks, store, 5, rope_mode="fp32", use_graph=False, **kw)
+    assert len(rows_seen) >= lw.num_layers and all(rows_seen)
+    rows_seen.clear()
+    run(lw, chunks, store, 5, use_graph=False, **kw)          # the default differs, or this test shows nothing
+    assert rows_seen and not all(rows_seen)
