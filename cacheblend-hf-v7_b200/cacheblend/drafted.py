@@ -162,14 +162,15 @@ def generate_drafted(layerwise_model, chunks: list[Chunk], kv_store: KVStore, ma
                               rope_mode, status, return_logits, use_graph, **options)
         n = len(out[0] if return_logits else out)
         return ((*out, n) if return_logits else (out, n)) if return_steps else out
-    vocab = lw.model.config.vocab_size
     out_rows: list[torch.Tensor] = []
     with torch.inference_mode():
-        choice = _Choice(lw.device, vocab, chunks, max_new_tokens + max_nodes, **options,
-                         status=status)
+        choice = _Choice(lw, chunks, max_new_tokens + max_nodes, **options, status=status)
         # the last step may check nodes past the last token asked for
         pre = _selective_prefill(lw, chunks, kv_store, recompute_ratio, check_layer, rope_mode, status, None,
                                  extra_tokens=max_new_tokens + max_nodes, logits_rows="last")
+        # what a drafted token may be: it is embedded, and may be chosen
+        vocab = pre.logits.shape[-1]
+        vocab = min(vocab, getattr(lw._inner.embed_tokens, "num_embeddings", vocab))
         row, first = choice(pre.logits[0, -1:], return_logits)
         out = [int(first.item())]
         if return_logits:

@@ -25,15 +25,22 @@ from cacheblend.fusor import _MLPS, _SILUS, _fused_w, _mlp, _norm, _qkv, _select
 from cacheblend.kv_store import KVStore
 
 
+def _vocab_size(model) -> int:
+    """Entries of a logits row: the configuration's, or the head's outputs."""
+    n = getattr(model.config, "vocab_size", None)
+    return model.lm_head.out_features if n is None else n
+
+
 class _Choice:
     """How a decode chooses tokens: penalties over the prompt's and the made
     tokens, bias and allowed tokens (``process_logits``), or plain argmax when
     none is asked for.  Holds the token history on the device: ``history[:length]``
     are the tokens so far, the first ``n_prompt`` of them the prompt's."""
 
-    def __init__(self, device, vocab: int, chunks: list[Chunk], spare: int, repetition_penalty: float,
-                 presence_penalty: float, frequency_penalty: float, logit_bias: torch.Tensor | None,
-                 allowed_tokens: torch.Tensor | None, status: torch.Tensor | None):
+    def __init__(self, lw, chunks: list[Chunk], spare: int, repetition_penalty: float, presence_penalty: float,
+                 frequency_penalty: float, logit_bias: torch.Tensor | None, allowed_tokens: torch.Tensor | None,
+                 status: torch.Tensor | None):
+        device = lw.device
         self.penalties = dict(repetition=float(repetition_penalty), presence=float(presence_penalty),
                               frequency=float(frequency_penalty))
         if not 0 < repetition_penalty < float("inf"):
@@ -41,6 +48,8 @@ class _Choice:
         self.counted = (repetition_penalty, presence_penalty, frequency_penalty) != (1.0, 0.0, 0.0)
         self.status = status
         self.bias = self.mask = None
+        # (looked up only for the options that need it)
+        vocab = None if logit_bias is None and allowed_tokens is None else _vocab_size(lw.model)
         if logit_bias is not None:
             if logit_bias.numel() != vocab:
                 raise ValueError(f"logit_bias must have {vocab} entries, got {logit_bias.numel()}")
@@ -200,8 +209,8 @@ def generate_greedy(layerwise_model, chunks: list[Chunk], kv_store: KVStore, max
     selective = 0 < recompute_ratio < 1 and len(chunks) > 1
     tokens, rows = [], []
     with torch.inference_mode():
-        choice = _Choice(lw.device, lw.model.config.vocab_size, chunks, max_new_tokens, repetition_penalty,
-                         presence_penalty, frequency_penalty, logit_bias, allowed_tokens, status)
+        choice = _Choice(lw, chunks, max_new_tokens, repetition_penalty, presence_penalty, frequency_penalty,
+                         logit_bias, allowed_tokens, status)
         if not selective:
             out = fuse_selective(lw, chunks, kv_store, recompute_ratio, check_layer, return_layerwise_output=True)
             row = out.logits[0, -1]

@@ -40,3 +40,31 @@ def test_decode_rotates_in_the_mode_asked_for(drafted, monkeypatch):
     rows_seen.clear()
     run(lw, chunks, store, 5, use_graph=False, **kw)          # the default differs, or this test shows nothing
     assert rows_seen and not all(rows_seen)
+
+
+class BareConfig:
+    """A model configuration without vocab_size (as of a model around a language model)."""
+
+    def __init__(self, config):
+        self.__dict__["_config"] = config
+
+    def __getattr__(self, name):
+        if name == "vocab_size":
+            raise AttributeError(name)
+        return getattr(self._config, name)
+
+
+def test_decode_without_a_vocabulary_size(monkeypatch):
+    cb, lw, model, chunks, store = _setup()
+    vocab = model.config.vocab_size
+    base = [run(lw, chunks, store, 5) for run in (cb.generate_greedy, cb.generate_drafted)]
+    only = torch.zeros((vocab,), dtype=torch.bool)
+    only[5] = True
+    monkeypatch.setattr(model, "config", BareConfig(model.config))
+    assert [run(lw, chunks, store, 5) for run in (cb.generate_greedy, cb.generate_drafted)] == base
+    for run in (cb.generate_greedy, cb.generate_drafted):     # the head's rows are the vocabulary
+        assert run(lw, chunks, store, 3, allowed_tokens=only) == [5, 5, 5]
+        with pytest.raises(ValueError):
+            run(lw, chunks, store, 3, logit_bias=torch.zeros(3))
+    with pytest.raises(ValueError):
+        cb.generate_drafted(lw, chunks, store, 3, draft=lambda ids, n: ([vocab], [-1]))
