@@ -58,6 +58,8 @@ class _Choice:
             if allowed_tokens.dtype != torch.bool or allowed_tokens.numel() != vocab:
                 raise ValueError(f"allowed_tokens must be bool with {vocab} entries, got "
                                  f"{allowed_tokens.dtype}{list(allowed_tokens.shape)}")
+            if not bool(allowed_tokens.any()):
+                raise ValueError("allowed_tokens allows no token")
             self.mask = ops.mask_words(allowed_tokens).to(device)
         self.plain = not self.counted and self.bias is None and self.mask is None
         if self.counted:
@@ -201,8 +203,9 @@ def generate_greedy(layerwise_model, chunks: list[Chunk], kv_store: KVStore, max
     of tokens that the prompt or the output has; ``frequency_penalty`` (per
     occurrence) and ``presence_penalty`` are taken off those that the output has.
     Then ``logit_bias`` (fp32, one per vocabulary entry) is added, and tokens
-    outside ``allowed_tokens`` (bool, one per entry) are excluded.  The returned
-    rows are those that chose, with all of this done."""
+    outside ``allowed_tokens`` (bool, one per entry, at least one set) are excluded;
+    where infinite penalties or biases leave only -inf, token 0 is chosen.  The
+    returned rows are those that chose, with all of this done."""
     if max_new_tokens <= 0:
         return ([], []) if return_logits else []
     lw = layerwise_model
