@@ -187,13 +187,12 @@ def generate_drafted(layerwise_model, chunks: list[Chunk], kv_store: KVStore, ma
                 raise ValueError(f"draft returned a token outside the vocabulary of {vocab}")
             tokens, parents = [out[-1], *drafted], [-1, *(p + 1 for p in below)]
             st.load(n_ctx, tokens, parents)
+            if use_graph and steps > 1 and graph is None:
+                graph = _capture(lw, pre, st, choice, rope_mode, status)
             if graph is not None:
                 graph.replay()
             else:
-                _tree_step(lw, pre, st, choice, rope_mode, status)   # eager: first use sets up every kernel
-                if use_graph and len(out) + 1 < max_new_tokens:
-                    graph = _capture(lw, pre, st, choice, rope_mode, status)
-                    graph.replay()                                     # (the same nodes again: the same result)
+                _tree_step(lw, pre, st, choice, rope_mode, status)     # eager: first use sets up every kernel
             chosen = st.chosen.tolist()
             path = _accept(tokens, parents, chosen)
             _keep(pre, choice, n_ctx, path, tokens)

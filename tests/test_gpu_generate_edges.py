@@ -68,3 +68,21 @@ def test_decode_without_a_vocabulary_size(monkeypatch):
             run(lw, chunks, store, 3, logit_bias=torch.zeros(3))
     with pytest.raises(ValueError):
         cb.generate_drafted(lw, chunks, store, 3, draft=lambda ids, n: ([vocab], [-1]))
+
+
+def test_every_step_runs_once(monkeypatch):
+    """A run of k decoder steps after the prefill: the first eagerly, the others as
+    k - 1 replays of its capture; none is run again for its result."""
+    cb, lw, model, chunks, store = _setup()
+    replays = []
+    replay = torch.cuda.CUDAGraph.replay
+    monkeypatch.setattr(torch.cuda.CUDAGraph, "replay", lambda g: (replays.append(g), replay(g))[1])
+    for length in (2, 3, 6):
+        replays.clear()
+        none = lambda ids, k: ([], [])
+        tokens, rows, steps = cb.generate_drafted(lw, chunks, store, length, draft=none, return_logits=True,
+                                                  return_steps=True)
+        assert len(tokens) == len(rows) == length == steps and len(replays) == length - 2
+        eager, eager_rows = cb.generate_drafted(lw, chunks, store, length, draft=none, return_logits=True,
+                                                use_graph=False)
+        assert tokens == eager and all(torch.equal(a, b) for a, b in zip(rows, eager_rows))
