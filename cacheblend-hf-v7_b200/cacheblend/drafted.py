@@ -183,6 +183,8 @@ def generate_drafted(layerwise_model, chunks: list[Chunk], kv_store: KVStore, ma
             if len(drafted) > max_nodes - 1 or len(drafted) != len(below):
                 raise ValueError(f"draft returned {len(drafted)} tokens and {len(below)} parents for {max_nodes - 1} "
                                  "nodes")
+            if any(p < -1 for p in below):
+                raise ValueError(f"draft returned parent {min(below)} (-1 or an earlier drafted token)")
             if any(not 0 <= t < vocab for t in drafted):
                 raise ValueError(f"draft returned a token outside the vocabulary of {vocab}")
             tokens, parents = [out[-1], *drafted], [-1, *(p + 1 for p in below)]

@@ -86,3 +86,10 @@ def test_every_step_runs_once(monkeypatch):
         eager, eager_rows = cb.generate_drafted(lw, chunks, store, length, draft=none, return_logits=True,
                                                 use_graph=False)
         assert tokens == eager and all(torch.equal(a, b) for a, b in zip(rows, eager_rows))
+
+
+def test_draft_parents_outside_the_tree_are_refused():
+    cb, lw, model, chunks, store = _setup()
+    for below in ([-2], [1], [-1, -2], [-1, 1]):
+        with pytest.raises(ValueError):
+            cb.generate_drafted(lw, chunks, store, 3, draft=lambda ids, n: ([4] * len(below), below))
