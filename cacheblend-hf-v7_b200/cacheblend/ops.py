@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 from typing import Sequence
 
 import numpy as np
@@ -507,7 +508,10 @@ def _launcher(name: str, n_launches: int):
 
     def launch(dev: torch.device, *args) -> None:
         index = dev.index
-        packed = pack(size, *args)
+        try:
+            packed = pack(size, *args)
+        except (OverflowError, struct.error) as e:
+            raise ValueError(f"{entry}: an argument does not fit its field ({e})") from None
         if TIMES.active or current_device() != index:
             with torch.cuda.device(dev), TIMES.span(name, dev, n_launches):
                 rc = fn(packed, raw_stream(index))
