@@ -93,3 +93,33 @@ def test_draft_parents_outside_the_tree_are_refused():
     for below in ([-2], [1], [-1, -2], [-1, 1]):
         with pytest.raises(ValueError):
             cb.generate_drafted(lw, chunks, store, 3, draft=lambda ids, n: ([4] * len(below), below))
+
+
+def forced(vocab, n, first=100):
+    """(tokens, options) such that every decode chooses these n tokens in turn: biases
+    100 apart, far above any logit, and a presence penalty that takes a token out once
+    it is made."""
+    tokens = [first + 3 * i for i in range(n)]
+    bias = torch.zeros((vocab,))
+    bias[tokens] = 4000.0 + 100.0 * n - 100.0 * torch.arange(n)
+    return tokens, dict(logit_bias=bias, presence_penalty=20000.0)
+
+
+@pytest.mark.parametrize("use_graph", [True, False])
+def test_ends_inside_an_accepted_path(use_graph):
+    """15 drafted nodes with two wrong siblings before each right one are 5 right
+    nodes, so a step gives 6 tokens: ends by count and by EOS at each place of a path."""
+    cb, lw, model, chunks, store = _setup(CFG128, n_chunks=4, chunk_len=100, q_len=20, seed=6)
+    answer, options = forced(CFG128["vocab_size"], 24)
+    n = sum(c.length for c in chunks)
+    kw = dict(return_logits=True, return_steps=True, use_graph=use_graph, max_nodes=16,
+              draft=oracle_draft(answer, n, [1, 7]), **options)
+    for length in (1, 2, 6, 7, 8, 10, 13, 14, 20):
+        tokens, rows, steps = cb.generate_drafted(lw, chunks, store, length, **kw)
+        assert tokens == answer[:length] and steps == 1 + (length - 1 + 5) // 6
+        assert [int(r.argmax()) for r in rows] == tokens
+    for at in (0, 1, 3, 6, 7, 9, 12, 17):
+        tokens, rows, steps = cb.generate_drafted(lw, chunks, store, 20, eos_token_id=answer[at], **kw)
+        assert tokens == answer[:at + 1] and steps == 1 + (at + 5) // 6
+        assert [int(r.argmax()) for r in rows] == tokens
+    assert cb.generate_greedy(lw, chunks, store, 20, eos_token_id=answer[9], **options) == answer[:10]
