@@ -580,9 +580,10 @@ def norm_rope_scatter(q_src: torch.Tensor, k_src: torch.Tensor, v_src: torch.Ten
     [n][Hq*D].
 
     q_src / k_src / v_src: n rows of heads (views of one stacked projection are
-    read in place; q_out must not overlap them); ``positions`` and ``rows``: int64, n entries -- siblings of a
-    drafted tree share a position, not a row; rows are distinct, and a row of -1
-    marks a padding token of which nothing is written.  ``rope``: fp32 (cos, sin)
+    read in place; q_out and the caches must not overlap them); ``positions`` and
+    ``rows``: int64, n entries -- siblings of a drafted tree share a position, not a
+    row; rows are distinct, and a row of -1 marks a padding token of which nothing is
+    written.  ``rope``: fp32 (cos, sin)
     table [n_pos][R / 2][2]; the first R dimensions of a head are rotated, as the
     pairs (i, i + R / 2) or, ``interleaved``, (2i, 2i + 1).  k_cache / v_cache:
     [cap][Hkv*D].  ``mode`` "ref" rounds to 16 bits where the HF modules do, "fp32"

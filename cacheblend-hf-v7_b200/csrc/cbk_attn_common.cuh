@@ -149,9 +149,9 @@ __device__ __forceinline__ void exp2_fma_pair(float x0, float x1, float& y0, flo
 
 // P = 2^(s * sl2 - m) of columns [32 c4, 32 c4 + 32) of a row, packed into 16-bit
 // pairs, with the row sum accumulated in packed fp32 pairs.  3 of the 16 pairs go
-// to the FMA-pipe polynomial.  Invisible keys arrive as s = -inf: ex2.approx gives
+// to the FMA-pipe polynomial (which drops a NaN argument).  Invisible keys arrive as s = -inf: ex2.approx gives
 // 0 for them, the polynomial (its argument clamped at -126) 2^-126; with EMU = 0
-// every pair takes ex2.approx, and their weight is 0 exactly.
+// every pair takes ex2.approx, their weight is 0 exactly and NaN stays NaN.
 template <int DT, unsigned EMU = CBK_ATTN_EMU_MASK>
 __device__ __forceinline__ void exp_chunk(const uint32_t (&s)[kBN], int c4, float sl2, float neg_m,
                                           float& ra0, float& ra1, float& rb0, float& rb1, uint32_t (&pk)[16]) {

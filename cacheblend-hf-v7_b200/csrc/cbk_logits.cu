@@ -21,8 +21,10 @@
 // keys (order of x, then lowest index) in the CTA and over the cluster, so no order of
 // atomics shows.  Rows that do not lie on 16-byte boundaries are read element by
 // element, neighbouring lanes on neighbouring elements.  64 rows of 128256 after 24 K
-// tokens: 26 us, bound by instructions and latency (its bytes would take 5.3); 16 rows
-// after 5 K 14, one row of 32000 after 6 K 5.9.
+// tokens with tree, mask and bias: 26 us, bound by instructions and latency (its bytes
+// would take 5.3); 16 rows after 5 K with tree and mask 14, one row of 32000 after 6 K 6.
+// Penalties alone, 64 rows of 128256 after 24 K tokens: 23.3 us, 22.7 when no logits are
+// written; 64 rows with a history of 5 K each 39.1 (every cluster counts), of 32000 22.1.
 //
 // Penalties come element by element, each behind a branch, or, with a history long for
 // its vocabulary (DENSE), for a whole vector in packed pairs without branches.
@@ -47,14 +49,20 @@ constexpr int kLgMaxVocab = 458752;
 constexpr int kLgMaxTree = 1024;
 constexpr int kLgMaxSmem = 224 * 1024;
 constexpr int kLgCountCtas = 8;                         // CTAs that count a shared history
-// Rows from which a shared history is counted once (64 rows of 128256 after 24 K
-// tokens: 29.6 us against 52.9 with every cluster counting; 16 rows after 5 K: 14.5
-// against 14.1), and clusters that fit side by side, two CTAs to an SM.
+// Rows from which a shared history is counted once, and clusters of 8 and of 4 that fit
+// side by side, two CTAs to each of 148 SMs (another number of SMs changes the time alone).
+// Counted by every cluster against once, us, penalties alone: 128256 tokens after 30000
+// 16 rows 23.8 / 16.4, 28 rows 24.2 / 16.8, 64 rows 43.4 / 24.1; after 5000 16 rows 13.3 /
+// 13.7, 28 rows 13.8 / 14.6, 32 rows 22.4 / 18.2; after 600 16 rows 10.3 / 11.9, 28 rows
+// 10.8 / 12.7, 32 rows 17.6 / 14.8; 32000 tokens after 500 28 rows 6.7 / 7.9, 32 rows
+// 10.1 / 8.6.  Beyond kLgFit8 rows once always wins; up to it the history's length
+// decides, which lies on the device, and 24 takes some of either.
 constexpr int kLgManyRows = 24, kLgFit8 = 30, kLgFit4 = 66;
 // A history's room over the vocabulary from which a vector's penalties are computed in
-// pairs, seen or not, instead of each behind a branch (64 rows of 128256: a history of
-// 24 K tokens 25.3 us with branches, 23.2 without, 12 K 23.3 and 22.7, 6 K 21.1 and 22.4,
-// 3 K 19.5 and 21.9; one row of 32000 after 6 K 6.6 and 6.0).
+// pairs, seen or not, instead of each behind a branch (penalties alone, 64 rows of 128256: a
+// history of 24 K tokens 25.3 us with branches, 23.2 without, 12 K 23.3 and 22.7, 6 K 21.1
+// and 22.4, 3 K 19.5 and 21.9; one row of 32000 after 6 K 6.6 and 6.0).  The room alone is
+// known to the host: a short history in much room pays the difference.
 constexpr int kLgDense = 16;
 constexpr uint32_t kLgPrompt = 0x80000000u;
 

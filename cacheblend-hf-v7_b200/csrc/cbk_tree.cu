@@ -38,17 +38,20 @@
 //
 // Visible keys: every exponential is ex2.approx, which keeps NaN and gives 0 for -inf.
 // exp_chunk's polynomial for 3 of 16 pairs clamps its argument, so a NaN score would
-// have weight 2^-126 there and an infinite one another than elsewhere; here it also gains
-// nothing (24 nodes over 131072 keys of 32 / 8 heads of 128: 92.7 us with, 92.8 without;
-// 64 over 32768: 43.3 and 43.1; 7 over 32768 of 14 / 2 heads of 64: 20.9 and 20.9).
+// have weight 2^-126 there and an infinite one another than elsewhere.  Here the
+// polynomial is slower too, since context and tree tiles would need code of their own
+// (32 q heads on 8 KV heads of 128: 64 nodes over 32768 keys 43.3 us with it, 40.9
+// without, 16 over 6208 13.4 and 13.2, 24 over 131072 90.8 and 90.9; 24 over 131072, 14
+// on 2 heads of 64, 40.4 and 38.8).
 //
 // Measured, 32 q heads on 8 KV heads of 128, bf16, both kernels of the call: 24 nodes over
-// 131072 keys 92 us (537 MB: 5.85 TB/s, 0.90 of measured HBM; 99 us in a long loop), 1
+// 131072 keys 90 us (537 MB: 5.97 TB/s, 0.91 of measured HBM; 95 us in a long loop), 1
 // node 86 us (6.2 TB/s);
-// 64 nodes (two Q tiles) over 32768 keys 43 us (790 TFLOP/s with both products counted: a
-// key tile takes both slots 1.9 us, of which the exponentials alone 1.3); 16 nodes over
-// 6208 keys 13.5 us, 1 node 10.5 (HBM alone 3.9: set-up 1.5, key tiles 3.3, epilogue 1,
-// merge launch and merge 3.5).
+// 64 nodes (two Q tiles) over 32768 keys 41 us (840 TFLOP/s with both products counted),
+// over 16384 28.6: a key tile takes both slots 1.7 us, of which its bytes would take 1.44
+// and its 32768 exponentials, 16 a clock, 1.04; 16 nodes over 6208 keys 13.1 us, 1 node
+// 10.1 (HBM alone 3.9; traced at 10.8 us: set-up 1.5, key tiles 3.3, epilogue 1, merge
+// launch and merge 3.5).
 // Every wait is bounded; on timeout the kernel sets CBK_STATUS_TIMEOUT, drains its
 // copies and MMAs, frees TMEM and returns.
 #include <algorithm>
@@ -128,12 +131,11 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
 
 template <int HD, int NQ>
 struct TreeSmem {
-  // K and V tiles in flight.  One Q tile, heads of 128: 3 against 2 is 17.1 against 17.7
-  // us for 8 nodes over 12000 keys, 93 against 100 for 24 over 131072 in a long loop (in
-  // a short one 91.3 against 90.5) and 13.4 against 12.6 for 16 over 6208; heads of 64:
-  // 3 against 6 is 16.9 against 18.0 for 7 nodes over 32768, 40.8 against 41.6 for 24
-  // over 131072.  Two Q tiles: 3 do not fit with heads of 128; heads of 64, 64 nodes
-  // over 16384: 18.9 with 2, 19.1 with 3 or 5.
+  // K and V tiles in flight.  One Q tile, 32 q heads on 8 KV heads of 128: 3 against 2 is
+  // 90.9 against 91.6 us for 24 nodes over 131072 keys, 10.1 against 10.2 for 1 over 6208,
+  // but 13.2 against 12.4 for 16 over 6208; 14 on 2 heads of 64, 24 over 131072: 39.5 with
+  // 2, 38.8 with 3 and with 4, 38.9 with 6.  Two Q tiles: 3 do not fit with heads of 128;
+  // 32 on 8 heads of 64, 64 over 16384: 24.3 to 26.6 with 2, 3 and 5, no order among them.
   static constexpr int kStages = NQ == 1 ? 3 : 2;
   static constexpr int kQBytes = kBM * HD * 2;
   static constexpr int kKVBytes = kBN * HD * 2;
@@ -698,8 +700,10 @@ static int launch_tree(const cbk_tree_attn_args* a, const TreeParams& p, cudaStr
 template <int DT>
 static int dispatch_tree(const cbk_tree_attn_args* a, const TreeParams& p, cudaStream_t st) {
   // One Q tile in both slots or two: the first could run as the second with one tile,
-  // but takes less room and is faster alone (7 nodes of 7 heads of 64 over 32768 keys
-  // 16.9 us against 17.4, 37 nodes over 1029 7.2 against 7.4).
+  // but takes half the workspace and has room for a third stage (24 nodes over 131072
+  // keys, 14 on 2 heads of 64: 38.8 us against 39.2; 37 over 1029, 4 on 2 heads of 64, 7.1
+  // against 7.4; 24 over 131072, 32 on 8 heads of 128, 90.9 against 90.6; 16 over 6208,
+  // which likes two stages better, 13.2 against 12.4).
   if (a->head_dim == 128) return p.n_qt == 1 ? launch_tree<DT, 128, 1>(a, p, st) : launch_tree<DT, 128, 2>(a, p, st);
   return p.n_qt == 1 ? launch_tree<DT, 64, 1>(a, p, st) : launch_tree<DT, 64, 2>(a, p, st);
 }

@@ -271,8 +271,8 @@ int cbk_scatter_rows(const void* src, int64_t src_stride_bytes, const int64_t* i
  *     (2i, 2i + 1); dimensions from rotary_dim on are not rotated
  *   q_out[j] = q, k_cache[r] = k, v_cache[r] = v_src[j]
  * rope_table: float2[table_rows][rotary_dim / 2].  Source and cache row strides
- * in elements; q_out is [n][n_q_heads * head_dim] and must not overlap a source.
- * rope_mode: CBK_ROPE_REF rounds to 16 bits where the HF modules do,
+ * in elements; q_out is [n][n_q_heads * head_dim]; neither it nor a cache may
+ * overlap a source.  rope_mode: CBK_ROPE_REF rounds to 16 bits where the HF modules do,
  * CBK_ROPE_FP32 once.  A row of -1 marks a padding token (nothing of it is
  * written); any other position or row outside its buffer sets
  * CBK_STATUS_BAD_INDEX and skips the token.  Rows are distinct (of two tokens with
@@ -299,8 +299,9 @@ int cbk_norm_rope_scatter(const cbk_norm_rope_scatter_args* args, void* stream);
  *   out[i][h] = softmax_t(scale * q[i][h] . k[t][h / G]) . v[t][h / G]
  * q, out: [n_nodes][n_q_heads][head_dim]; caches: cap rows of kv_row_stride
  * elements, head h at h * head_dim; words: rows of words_stride int32.  A node
- * that sees no row gets zeros.  What a masked row holds (NaN and infinities
- * included) and rows from *n_ctx + n_nodes on do not matter.  *n_ctx is read on
+ * that sees no row gets zeros; a visible score of NaN or +inf makes its row NaN, one of
+ * -inf has weight 0 (NaN, as 0 / 0, where a row sees no other).  What a masked row holds
+ * (NaN and infinities included) and rows from *n_ctx + n_nodes on do not matter.  *n_ctx is read on
  * the device (a captured graph stays valid as it advances); *n_ctx < 0 or
  * *n_ctx + n_nodes > cap sets CBK_STATUS_BAD_INDEX and leaves out untouched.
  * head_dim 64 or 128, n_nodes <= 1024, any whole number of q heads per KV head;
